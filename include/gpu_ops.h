@@ -15,7 +15,8 @@
  *   - all arguments are validated on the host before anything is launched; no
  *     kernel traps or asserts;
  *   - `dt` is the reference's DataType value: 4 = fp16, 5 = bf16
- *     (prebuild/defs.hpp:8-18).  Accumulation is always fp32.
+ *     (prebuild/defs.hpp:8-18).  Accumulation is always fp32.  The cache may be
+ *     held in 8 bits (gpu_kv_q8).
  *
  * All pointers are device pointers unless a parameter is documented as host
  * memory.  Calls are asynchronous on `stream`.  head_dim must be 128 (every
@@ -368,6 +369,93 @@ int gpu_attn_decode_paged_layer(const gpu_attn_desc *desc, const gpu_kv_pages *p
                                 const int32_t *kv_len_dev, int append_new, int max_kv_len,
                                 void *workspace, size_t workspace_bytes, gpu_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * 8-bit KV cache.  The reference keeps K and V in the activation type
+ * (src/llama2_layer_npu.cpp:1148-1149); these operators hold them in 8 bits, so
+ * that a decode step reads half the bytes and a GPU holds twice the tokens.  A
+ * cache row -- one position of one KV head, 128 elements -- is 128 e4m3 codes and
+ * one exponent byte x:
+ *     value = code * 2^(x - 127)
+ * with the smallest exponent >= -100 for which the row's largest magnitude is at
+ * most 448 * 2^(x - 127).  A power of two costs a floating format no precision,
+ * applies without rounding, and fits in a byte.  Rows are quantised from the fp32
+ * rotated K and from V with one rounding (to nearest even).  A row that holds a
+ * value that is not finite is stored with x = 255 and reads as NaN; every query
+ * row that sees it gets a NaN output, the others do not.  Codes 0x7F and 0xFF
+ * (NaN) are never written, and the operators expect none in positions they read.
+ *
+ * Batches are ragged: the rows of the sequences' new tokens follow one another,
+ * sequence b owns rows tok_start[b] .. tok_start[b + 1] - 1 (int32 [batch + 1] on
+ * the device, non-decreasing, 0 <= entries <= total_tokens; a sequence may have
+ * none), and row r of them stands at cache position start_pos[b] + r.  Token rows
+ * are addressed by the descriptor's *_tok_stride; *_seq_stride is used by the
+ * decode operator only, which takes one row per sequence.  Rows at and beyond
+ * tok_start[batch] are neither read nor written.
+ *
+ * All lengths and tables are read on the device when the kernel runs, so that a
+ * captured graph may be replayed after they have changed.  A position outside
+ * [0, max_pos) or a page id outside the pool is skipped (written nowhere; read as
+ * the rows of page 0) and reported by gpu_ops_kernel_status() == 41, a length
+ * beyond the host's bound == 40.
+ * ------------------------------------------------------------------------ */
+
+/* The cache.  Codes follow the descriptor's cache strides (an element is a byte;
+ * all strides multiples of 16) and, over pages, page_stride; exponents of row
+ * (b or page, kv_head, pos) lie at b_or_page*exp_outer_stride +
+ * kv_head*exp_head_stride + pos, both strides multiples of 16.  Without pages a
+ * sequence's cache holds max_pos positions (exponent rows padded to a multiple of
+ * 16); over pages max_pos <= table_stride * page_size.  RoPE tables have at least
+ * max_pos rows.  All four pointers 16-byte aligned. */
+typedef struct gpu_kv_q8 {
+  void *k, *v;                       /* e4m3 codes */
+  uint8_t *k_exp, *v_exp;            /* exponent bytes */
+  int64_t exp_outer_stride, exp_head_stride;
+  int32_t max_pos;
+  int32_t reserved;                  /* 0 */
+} gpu_kv_q8;
+
+/* RoPE(Q) -> q_out, RoPE(K) -> 8-bit cache, V -> 8-bit cache for the new tokens
+ * of a ragged batch; pages: NULL for a flat cache.  q_in / q_out rows are
+ * q_tok_stride apart (q_out may alias q_in; NULL: Q is not touched), k_in / v_in
+ * rows kv_in_tok_stride apart.  start_pos_dev: int32 [batch]. */
+int gpu_rope_kv_append_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv,
+                                void *q_out, const void *q_in, const void *k_in, const void *v_in,
+                                const void *freqs_cis_dev, const int32_t *tok_start_dev,
+                                const int32_t *start_pos_dev, int total_tokens, gpu_stream_t stream);
+
+/* The way back: rows of the 8-bit cache -> k_out / v_out [rows][n_kv_heads][128]
+ * in the descriptor's type, rows kv_in_tok_stride apart; the rows of sequence b
+ * are the positions from start_pos[b] on (start_pos_dev NULL: from 0).  Either
+ * output may be NULL. */
+int gpu_kv_read_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *k_out,
+                         void *v_out, const int32_t *tok_start_dev, const int32_t *start_pos_dev,
+                         int total_tokens, gpu_stream_t stream);
+
+/* Attention of one (already rotated) query row per sequence over the first
+ * kv_len[b] positions of its 8-bit cache -- the token's own K and V are in it.
+ * With window > 0 the row sees the last `window` positions and the first n_sink
+ * ones; window 0: all.  Pages without a visible position are not touched (their
+ * table entries may be stale).  kv_len 0 gives a zero row.  n_heads / n_kv_heads
+ * at most 16.  max_kv_len: host upper bound of kv_len.  workspace: device scratch of at least
+ * gpu_attn_decode_q8_workspace_bytes(), not shared by calls that may overlap; its
+ * contents need not be cleared. */
+int gpu_attn_decode_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *out,
+                             const void *q, const int32_t *kv_len_dev, int max_kv_len, int window, int n_sink,
+                             void *workspace, size_t workspace_bytes, gpu_stream_t stream);
+size_t gpu_attn_decode_q8_workspace_bytes(const gpu_attn_desc *desc, int max_kv_len);
+
+/* Causal attention of a ragged batch's new (already rotated, already appended)
+ * tokens over their 8-bit caches: row r of sequence b stands at position
+ * start_pos[b] + r and sees the positions up to its own, with `window` and n_sink
+ * as above.  max_new: host upper bound of the new tokens of a sequence;
+ * max_kv_len: of start_pos[b] + new tokens.  Rows of sequences that bring no token
+ * do not exist; rows beyond the last sequence stay as they were. */
+int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *out,
+                            const void *q, const int32_t *tok_start_dev, const int32_t *start_pos_dev,
+                            int total_tokens, int max_new, int max_kv_len, int window, int n_sink,
+                            void *workspace, size_t workspace_bytes, gpu_stream_t stream);
+size_t gpu_attn_chunk_q8_workspace_bytes(const gpu_attn_desc *desc, int total_tokens, int max_new, int max_kv_len);
+
 /* Merge n_parts partial results: o_parts fp32 [n_parts][rows][head_dim]
  * (normalised), lse_parts fp32 [n_parts][rows] (natural log).
  * out[row] = sum_p exp(lse_p - M) o_p / sum_p exp(lse_p - M), M = max_p lse_p,
@@ -437,7 +525,8 @@ int gpu_attn_last_prefill_kernel(void);
  * the context usable; 40 = a sequence of gpu_attn_decode_layer was longer than
  * max_kv_len, so that its last positions -- the new token among them -- were not
  * covered (the output and cache of that sequence are wrong, nothing is read or
- * written out of bounds).  Read it after synchronising. */
+ * written out of bounds); 41 = a position or a page id of an 8-bit cache operator
+ * lay outside the cache.  Read it after synchronising. */
 int gpu_ops_kernel_status(void);
 /* Resets that status to 0 (call with no kernel of the library in flight on the device). */
 int gpu_ops_clear_kernel_status(void);

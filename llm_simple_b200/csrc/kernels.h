@@ -231,6 +231,63 @@ void attn_clear_error_status();
 // Device address of that status word (host-mapped), or nullptr.
 int *kernel_error_word_dev();
 
+// ---- 8-bit KV cache ------------------------------------------------------------
+// Codes: byte (outer, kv head, pos, d) at outer * c_outer + head * c_head + pos * c_pos + d; exponent
+// bytes at outer * x_outer + head * x_head + pos.  outer is the sequence, or the page with pos the
+// position inside it.
+struct Q8Cache {
+  uint8_t *k, *v, *kx, *vx;
+  long c_outer, c_head, c_pos;
+  long x_outer, x_head;
+  KvPaging pg;         // pg.table == nullptr: flat
+  int max_pos;         // positions a sequence can hold
+  int batch, n_kv_heads;
+  int *error_flag;     // status word (host-mapped)
+};
+// A position outside [0, max_pos) or a page id outside the pool was met.
+constexpr int kStatusOutsideCache = 41;
+
+// Rows of a ragged batch: sequence b owns rows tok_start[b] .. tok_start[b + 1] - 1, row r of them
+// stands at position start_pos[b] + r (start_pos == nullptr: r).
+struct Ragged {
+  const int32_t *tok_start, *start_pos;
+  int total;
+};
+
+struct Q8AppendParams {
+  Q8Cache c;
+  Ragged r;
+  void *q_out;         // or nullptr
+  const void *q, *k, *v;
+  const float *freqs_cis;
+  long q_tok, kv_tok;
+  int n_heads, is_neox;
+};
+cudaError_t launch_kv_append_q8(const Q8AppendParams &p, bool bf16, cudaStream_t stream);
+
+struct Q8ReadParams {
+  Q8Cache c;
+  Ragged r;
+  void *k_out, *v_out; // either may be nullptr
+  long kv_tok;
+};
+cudaError_t launch_kv_read_q8(const Q8ReadParams &p, bool bf16, cudaStream_t stream);
+
+struct Q8AttnParams {
+  Q8Cache c;
+  Ragged r;            // chunk form
+  const int32_t *kv_len; // decode form: one row per sequence at position kv_len[b] - 1; nullptr: chunk form
+  void *out;
+  const void *q;
+  long q_row, out_row; // elements between rows (decode: sequences; chunk: tokens)
+  int n_heads, group;
+  int max_kv_len, max_new;
+  int window, n_sink;  // window 0: unlimited
+  float scale_log2;
+  void *ws;
+};
+cudaError_t launch_attn_q8(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches);
+
 // ---- cross-device (O, LSE) exchange + merge over peer memory ------------------
 constexpr int kMaxPeers = 8;
 struct XchgParams {

@@ -1,0 +1,78 @@
+// Device helpers of the 8-bit KV cache: where a row lies, which sequence a token row belongs to, and
+// the e4m3 <-> 16-bit conversions.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace b200attn {
+namespace q8 {
+
+constexpr int kMinExp = -100;    // smallest row exponent
+constexpr int kPoison = 255;     // exponent byte of a row that holds a value that is not finite
+
+__device__ __forceinline__ void report(int *error_flag, int code) {
+  if (error_flag) *reinterpret_cast<volatile int *>(error_flag) = code;
+}
+
+// Outer index (sequence or page) and in-page position of position pos of sequence b; false if the
+// position or its page lies outside the cache.
+__device__ __forceinline__ bool locate(const Q8Cache &c, int b, int pos, long &outer, int &in_pos) {
+  if (static_cast<unsigned>(pos) >= static_cast<unsigned>(c.max_pos)) return false;
+  if (!c.pg.table) {
+    outer = b;
+    in_pos = pos;
+    return true;
+  }
+  const int page = __ldg(c.pg.table + static_cast<long>(b) * c.pg.table_stride + (pos >> c.pg.page_shift));
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pg.n_pages)) return false;
+  outer = page;
+  in_pos = pos & ((1 << c.pg.page_shift) - 1);
+  return true;
+}
+
+// Sequence of token row t: the number of entries tok_start[1 .. batch] that are <= t, found by the
+// eight threads of a group (`sub` 0 .. 7) together, eight probes a round.  All 32 lanes take part.
+// batch: the row lies behind the last sequence.
+__device__ __forceinline__ int seq_of_row(const int32_t *tok_start, int batch, int t, int lane) {
+  const int sub = lane & 7, shift = lane & 24;
+  int lo = 0, len = batch; // the count lies in [lo, lo + len]
+  while (__any_sync(0xffffffffu, len > 0)) {
+    const int step = (len + 7) >> 3;
+    const int idx = lo + step * (sub + 1);
+    const bool le = len > 0 && idx <= lo + len && __ldg(tok_start + idx) <= t;
+    const int k = __popc((__ballot_sync(0xffffffffu, le) >> shift) & 0xffu);
+    const int hi = min(lo + len, lo + step * (k + 1) - 1);
+    lo += step * k;
+    len = len > 0 ? max(0, hi - lo) : 0;
+  }
+  return lo;
+}
+
+// Two e4m3 codes (low half of `u`) -> two fp16 values, exact.
+__device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t u) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(u));
+  return r;
+}
+// Two fp32 values -> two e4m3 codes (a in the low byte), to nearest even.
+__device__ __forceinline__ uint32_t cvt_f32_e4m3x2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); } // -126 <= e <= 127
+
+// Exponent of a row whose largest magnitude is amax (finite): the smallest e >= kMinExp with
+// amax <= 448 * 2^e = 1.75 * 2^(e + 8).  Adding what lies between 1.75 and 2 to the mantissa carries
+// into the exponent field exactly when the mantissa is above 1.75.
+__device__ __forceinline__ int row_exp(float amax) {
+  const int e = static_cast<int>((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
+  return max(e, kMinExp);
+}
+
+// One query row's visible positions: [0, min(sink, lo)) and [lo, pos].
+__device__ __forceinline__ int window_begin(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
+
+} // namespace q8
+} // namespace b200attn

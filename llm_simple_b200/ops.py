@@ -27,6 +27,8 @@ EXPORTS = [
     "gpu_attn_xchg_buffer_bytes", "gpu_attn_xchg_local_slot", "gpu_attn_xchg_merge_layer",
     "gpu_attn_decode_xchg_layer",
     "gpu_peer_buffer_alloc", "gpu_peer_buffer_open", "gpu_peer_buffer_close", "gpu_peer_buffer_free",
+    "gpu_rope_kv_append_q8_layer", "gpu_kv_read_q8_layer", "gpu_attn_decode_q8_layer", "gpu_attn_decode_q8_workspace_bytes",
+    "gpu_attn_chunk_q8_layer", "gpu_attn_chunk_q8_workspace_bytes",
     "gpu_ops_set_workspace", "gpu_attn_set_decode_chunk", "gpu_attn_set_decode_early_prefetch", "gpu_attn_set_prefill_kernel", "gpu_attn_set_prefill_l2_window", "gpu_attn_last_prefill_kernel",
     "gpu_ops_launch_count", "gpu_ops_last_error_string", "gpu_ops_kernel_status", "gpu_ops_clear_kernel_status",
 ]
@@ -52,6 +54,26 @@ def make_pages(page_table, page_size, page_stride, n_pages):
     pg.n_pages = n_pages
     pg._keep = page_table
     return pg
+
+
+class KvQ8(ctypes.Structure):
+    """struct gpu_kv_q8 (include/gpu_ops.h): an 8-bit KV cache, e4m3 codes and one exponent byte per row."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p),
+                ("exp_outer_stride", ctypes.c_int64), ("exp_head_stride", ctypes.c_int64), ("max_pos", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+def make_kv_q8(k, v, k_exp, v_exp, max_pos):
+    """k, v: device byte tensors of the codes, in the layout the descriptor's cache strides (and the pages) say;
+    k_exp, v_exp: device uint8 tensors [batch or pages][kv heads][positions], last dimension dense."""
+    kv = KvQ8()
+    kv.k, kv.v, kv.k_exp, kv.v_exp = _ptr(k), _ptr(v), _ptr(k_exp), _ptr(v_exp)
+    if k_exp.stride(2) != 1 or k_exp.stride() != v_exp.stride():
+        raise ValueError("exponent tensors: equal strides, positions dense")
+    kv.exp_outer_stride, kv.exp_head_stride = k_exp.stride(0), k_exp.stride(1)
+    kv.max_pos = max_pos
+    kv._keep = (k, v, k_exp, v_exp)
+    return kv
 
 
 class AttnDesc(ctypes.Structure):
@@ -129,6 +151,15 @@ def lib():
                                                                                                  ctypes.c_size_t, vp]
         L.gpu_attn_decode_workspace_bytes.argtypes = [dp, i]
         L.gpu_attn_decode_workspace_bytes.restype = ctypes.c_size_t
+        kp = ctypes.POINTER(KvQ8)
+        L.gpu_rope_kv_append_q8_layer.argtypes = [dp, pp, kp] + [vp] * 5 + [i32p, i32p, i, vp]
+        L.gpu_kv_read_q8_layer.argtypes = [dp, pp, kp, vp, vp, i32p, i32p, i, vp]
+        L.gpu_attn_decode_q8_layer.argtypes = [dp, pp, kp, vp, vp, i32p, i, i, i, vp, ctypes.c_size_t, vp]
+        L.gpu_attn_decode_q8_workspace_bytes.argtypes = [dp, i]
+        L.gpu_attn_decode_q8_workspace_bytes.restype = ctypes.c_size_t
+        L.gpu_attn_chunk_q8_layer.argtypes = [dp, pp, kp, vp, vp, i32p, i32p, i, i, i, i, i, vp, ctypes.c_size_t, vp]
+        L.gpu_attn_chunk_q8_workspace_bytes.argtypes = [dp, i, i, i]
+        L.gpu_attn_chunk_q8_workspace_bytes.restype = ctypes.c_size_t
         L.gpu_attn_merge_lse_layer.argtypes = [vp, f32p, f32p, i, i, i, i, vp]
         L.gpu_attn_merge_packed_layer.argtypes = [vp, f32p, i, i, i, i, vp]
         L.gpu_attn_xchg_buffer_bytes.argtypes = [i, i]
@@ -385,6 +416,48 @@ def gpu_attn_decode_xchg_layer(desc, out, q_in, k_in, v_in, k_cache, v_cache, fr
                                             _ptr(k_cache), _ptr(v_cache), _ptr(freqs_cis), _ptr(kv_len_dev),
                                             _ptr(rope_pos_dev), int(bool(append_new)), max_kv_len, _ptr(workspace),
                                             workspace_bytes, local_buffer, arr, world, rank, epoch, _stream(stream)))
+
+
+def _ref(struct):
+    return None if struct is None else ctypes.byref(struct)
+
+
+def gpu_rope_kv_append_q8_layer(desc, pages, kv, q_out, q_in, k_in, v_in, freqs_cis, tok_start_dev, start_pos_dev,
+                                total_tokens, stream=None):
+    """RoPE + append of a ragged batch into an 8-bit cache (make_kv_q8); pages: None for a flat cache."""
+    _check(lib().gpu_rope_kv_append_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(q_out), _ptr(q_in),
+                                             _ptr(k_in), _ptr(v_in), _ptr(freqs_cis), _ptr(tok_start_dev),
+                                             _ptr(start_pos_dev), total_tokens, _stream(stream)))
+
+
+def gpu_kv_read_q8_layer(desc, pages, kv, k_out, v_out, tok_start_dev, start_pos_dev, total_tokens, stream=None):
+    """Rows of an 8-bit cache back in 16 bits, ragged; start_pos_dev None: from position 0."""
+    _check(lib().gpu_kv_read_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(k_out), _ptr(v_out),
+                                      _ptr(tok_start_dev), _ptr(start_pos_dev), total_tokens, _stream(stream)))
+
+
+def gpu_attn_decode_q8_workspace_bytes(desc, max_kv_len):
+    return int(lib().gpu_attn_decode_q8_workspace_bytes(ctypes.byref(desc), max_kv_len))
+
+
+def gpu_attn_decode_q8_layer(desc, pages, kv, out, q, kv_len_dev, max_kv_len, window, n_sink, workspace,
+                             workspace_bytes, stream=None):
+    """One rotated query row per sequence over its 8-bit cache; window 0: everything is visible."""
+    _check(lib().gpu_attn_decode_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(out), _ptr(q),
+                                          _ptr(kv_len_dev), max_kv_len, window, n_sink, _ptr(workspace),
+                                          workspace_bytes, _stream(stream)))
+
+
+def gpu_attn_chunk_q8_workspace_bytes(desc, total_tokens, max_new, max_kv_len):
+    return int(lib().gpu_attn_chunk_q8_workspace_bytes(ctypes.byref(desc), total_tokens, max_new, max_kv_len))
+
+
+def gpu_attn_chunk_q8_layer(desc, pages, kv, out, q, tok_start_dev, start_pos_dev, total_tokens, max_new, max_kv_len,
+                            window, n_sink, workspace, workspace_bytes, stream=None):
+    """Causal attention of a ragged batch's new, appended tokens over their 8-bit caches."""
+    _check(lib().gpu_attn_chunk_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(out), _ptr(q),
+                                         _ptr(tok_start_dev), _ptr(start_pos_dev), total_tokens, max_new, max_kv_len,
+                                         window, n_sink, _ptr(workspace), workspace_bytes, _stream(stream)))
 
 
 def gpu_attn_merge_lse_layer(out, o_parts, lse_parts, n_parts, rows, head_dim, dt, stream=None):
