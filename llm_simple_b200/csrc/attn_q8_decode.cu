@@ -1,0 +1,724 @@
+// Attention of a few query rows per sequence over the 8-bit KV cache: decode (one row per query head)
+// and short chunks with at most 16 rows per KV head.
+//
+// Every (sequence, KV head) cache is a run of tiles of 64 positions -- those that hold the first
+// visible positions and those from the window's begin to the last row; the runs are laid end to end
+// and every CTA takes an equal, contiguous share of that line.  The lengths are read on the device:
+// each CTA adds up the runs of the batch (a scan of `batch` integers, about a microsecond) and finds
+// its share, so a captured graph follows the lengths.  Six warps:
+//   warps 0-3  16 of a tile's 64 positions each: S = Q K^T and O += P V as mma.sync m16n8k16 on fp16.
+//              e4m3 converts to fp16 exactly, two codes an instruction, straight from the bytes of
+//              the tile: a lane's share of a K row is 32 consecutive bytes (the order of the 128
+//              elements in the contraction is free, as long as Q's is the same), and its share of V
+//              is 16 consecutive bytes of four rows, whose bytes two permutes pair up.
+//   warp 4     TMA producer: K and V tiles (128-byte swizzle) and their exponent bytes, 5 stages of
+//              16 KB
+//   warp 5     the piece's query rows, as fp16 scaled by a power of two (exact for bf16 and fp16)
+// The row exponents never touch the products.  With e_k, e_v those of a position,
+//     t = S 2^e_k scale log2(e) + e_v,   P = 2^(t - max t),   O += P c_v,   l += P 2^-e_v
+// and O / l is the attention: sums in fp32, P rounded to fp16 (11 bits; it is at most 2^8, since O is
+// rescaled only when the running maximum has grown by more than that).
+//
+// A run that lies in one share is written out; a run that was cut leaves a normalised partial and its
+// log-sum-exp per piece, merged by a second, dependent launch in a fixed order.
+//
+// HBM-bound: 258 bytes per visible position and KV head, read once.
+#include "q8.cuh"
+#include "tc5.cuh"
+#include "tma.cuh"
+
+namespace b200attn {
+
+namespace q8d {
+
+using namespace q8;
+using namespace tma;
+
+constexpr int kConsumerWarps = 4;
+constexpr int kConsumerThreads = kConsumerWarps * 32;
+constexpr int kThreads = kConsumerThreads + 64;
+constexpr int kStages = 5;
+constexpr int kTileN = 64;
+constexpr uint32_t kTile = kTileN * 128;             // K or V codes of a tile
+constexpr uint32_t kStageBytes = 2 * kTile;
+constexpr uint32_t kOffCombine = kStages * kStageBytes;              // [4 warps][8 rows][128] fp32
+constexpr uint32_t kOffExp = kOffCombine + kConsumerWarps * 8 * 512; // [stage][K, V][64]
+constexpr uint32_t kOffQ = kOffExp + kStages * 128;                  // [16][128] fp16
+constexpr uint32_t kOffQs = kOffQ + 16 * 256;                        // [16] fp32: what a row's scores are multiplied by
+constexpr uint32_t kOffMl = kOffQs + 64;                             // [4][16][max, sum]
+constexpr uint32_t kOffScan = kOffMl + kConsumerWarps * 16 * 8;      // scan scratch: 8 + 4 ints
+constexpr uint32_t kOffBar = kOffScan + 64;
+constexpr uint32_t kSmemTotal = kOffBar + 128;
+static_assert(kSmemTotal <= 115712, "two CTAs per SM");
+constexpr int kMaxCtas = 296;                        // two per SM
+constexpr float kLazy = 8.0f;                        // log2 of how far P may exceed 1 before O is rescaled
+
+enum { BAR_FULL = 0, BAR_EMPTY = kStages, BAR_QREADY = 2 * kStages, BAR_QFREE, BAR_COUNT };
+static_assert(BAR_COUNT * 8 + 8 <= 128, "barrier block");
+
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory"); }
+
+// One sequence's rows and the tiles they see.
+struct Seq {
+  int t0, nq;          // its first row and number of rows
+  int pos0;            // position of the first row
+  int end;             // one past the last visible position
+  int lo;              // first window position of the first row
+  int ns;              // first positions visible besides the window
+  int ns_tiles, w0, n_tiles; // tiles 0 .. ns_tiles - 1, then w0, w0 + 1, ...
+  __device__ __forceinline__ int tile(int i) const { return i < ns_tiles ? i : w0 + i - ns_tiles; }
+};
+
+__device__ __forceinline__ Seq seq_of(const Q8AttnParams &p, int b) {
+  Seq s;
+  const int limit = min(p.max_kv_len, p.c.max_pos);
+  if (p.kv_len) {
+    const int len = __ldg(p.kv_len + b);
+    if (len > limit) report(p.c.error_flag, kStatusLengthBeyondBound);
+    s.t0 = b;
+    s.nq = 1;
+    s.pos0 = min(len, limit) - 1;
+  } else {
+    const int a = min(max(__ldg(p.r.tok_start + b), 0), p.r.total), e = min(max(__ldg(p.r.tok_start + b + 1), a), p.r.total);
+    s.t0 = a;
+    s.nq = e - a;
+    s.pos0 = __ldg(p.r.start_pos + b);
+    if (s.nq > p.max_new) {
+      report(p.c.error_flag, kStatusLengthBeyondBound);
+      s.nq = p.max_new;
+    }
+    if (s.nq > 0) {
+      const long last = static_cast<long>(s.pos0) + s.nq - 1;
+      if (s.pos0 < 0 || last >= p.c.max_pos) report(p.c.error_flag, kStatusOutsideCache);
+      else if (last >= limit) report(p.c.error_flag, kStatusLengthBeyondBound);
+      s.pos0 = max(s.pos0, -32);
+    }
+  }
+  s.end = s.nq > 0 ? max(0, static_cast<int>(min(static_cast<long>(s.pos0) + s.nq, static_cast<long>(limit)))) : 0;
+  s.lo = min(window_begin(s.pos0, p.window), s.end);
+  s.ns = min(p.n_sink, s.lo);
+  s.ns_tiles = (s.ns + kTileN - 1) / kTileN;
+  s.w0 = max(s.lo / kTileN, s.ns_tiles);
+  s.n_tiles = s.end > 0 ? s.ns_tiles + max(0, (s.end + kTileN - 1) / kTileN - s.w0) : 0;
+  return s;
+}
+
+// Share c of a line of W tiles cut for n CTAs, and the CTA that owns tile x.
+__device__ __forceinline__ long share_begin(long W, int n, int c) { return static_cast<long>(c) * W / n; }
+__device__ __forceinline__ int share_of(long W, int n, long x) { return static_cast<int>(((x + 1) * n - 1) / W); }
+
+// The pieces of one CTA's share, in order.
+struct Walk {
+  int b, kvh, i0, i1;
+  long left;
+  Seq s;
+  __device__ __forceinline__ void begin(const Q8AttnParams &p, int b_, long offset, long tiles) {
+    b = b_;
+    s = seq_of(p, b);
+    kvh = static_cast<int>(offset / s.n_tiles);
+    i0 = static_cast<int>(offset - static_cast<long>(kvh) * s.n_tiles);
+    left = tiles;
+    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), i0 + left));
+  }
+  __device__ __forceinline__ bool next(const Q8AttnParams &p) { // false: the share is done
+    left -= i1 - i0;
+    if (left <= 0) return false;
+    if (++kvh == p.c.n_kv_heads) {
+      kvh = 0;
+      do {
+        if (++b >= p.c.batch) return false;
+        s = seq_of(p, b);
+      } while (s.n_tiles == 0);
+    }
+    i0 = 0;
+    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), left));
+    return true;
+  }
+};
+
+// A piece's partial goes to slot 2 c (the share's first piece) or 2 c + 1 (its last one).  Which slots
+// a cut run left: first and last CTA, and the slot of the first; of the others it is 2 c.
+struct RunInfo {
+  int c0, c1, slot0, pad;
+};
+
+struct Ws {
+  float *o, *lse; // [slot][rows][128], [slot][rows]
+  RunInfo *info;  // [batch * kv heads]
+};
+
+} // namespace q8d
+
+struct Q8DecodeParams {
+  Q8AttnParams a;
+  q8d::Ws ws;
+  int rows;       // rows of a partial: max_new * group
+  int min_tiles;  // smallest share worth a CTA
+};
+
+template <typename T, bool WIDE> // WIDE: more than 8 rows
+__global__ void __launch_bounds__(q8d::kThreads, 2)
+attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ CUtensorMap map_k16, const __grid_constant__ CUtensorMap map_v16, const Q8DecodeParams dp) {
+  using namespace q8d;
+  const Q8AttnParams &p = dp.a;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t smem_base = smem_u32(smem);
+  int *scan = reinterpret_cast<int *>(smem + kOffScan);
+  float *red_ml = reinterpret_cast<float *>(smem + kOffMl);
+  volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + kOffBar + BAR_COUNT * 8);
+  auto bar = [&](int i) { return smem_base + kOffBar + 8u * i; };
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = p.group, kvH = p.c.n_kv_heads;
+
+  cudaTriggerProgrammaticLaunchCompletion();
+  if (tid == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar(BAR_FULL + s), 1);
+      mbar_init(bar(BAR_EMPTY + s), kConsumerWarps);
+    }
+    mbar_init(bar(BAR_QREADY), 1);
+    mbar_init(bar(BAR_QFREE), kConsumerWarps);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  cudaGridDependencySynchronize(); // lengths, rows, cache and scratch may be the preceding kernels'
+
+  // ---- this CTA's share: tiles of the whole batch, and the sequence its first tile belongs to
+  const int per = (p.c.batch + kThreads - 1) / kThreads;
+  const int b_lo = min(p.c.batch, tid * per), b_hi = min(p.c.batch, b_lo + per);
+  int mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += seq_of(p, b).n_tiles;
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) scan[warp] = incl;
+  if ((smem_base & 1023u) != 0 && tid == 0) report(p.c.error_flag, 30);
+  __syncthreads();
+  if ((smem_base & 1023u) != 0) return;
+  int before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const long W = static_cast<long>(total) * kvH;
+  const int n = static_cast<int>(min(static_cast<long>(gridDim.x), (W + dp.min_tiles - 1) / dp.min_tiles));
+  const int c = blockIdx.x;
+  if (c >= n) return;
+  const long x0 = share_begin(W, n, c), x1 = share_begin(W, n, c + 1);
+  if (x0 >= static_cast<long>(before) * kvH && x0 < static_cast<long>(before + mine) * kvH) {
+    long at = static_cast<long>(before) * kvH;
+    for (int b = b_lo; b < b_hi; ++b) {
+      const long run = static_cast<long>(seq_of(p, b).n_tiles) * kvH;
+      if (x0 < at + run) {
+        scan[8] = b;
+        scan[9] = static_cast<int>(x0 - at);
+        break;
+      }
+      at += run;
+    }
+  }
+  __syncthreads();
+  const int b_first = scan[8], off_first = scan[9];
+
+  if (warp == kConsumerWarps) {
+    // ------------------------------------------------------------------ TMA producer
+    Walk w;
+    w.begin(p, b_first, off_first, x1 - x0);
+    uint32_t g = 0;
+    do {
+      for (int base = w.i0; base < w.i1; base += 32) {
+        // the lanes look up the pages of 32 tiles at once
+        const int mine_i = base + lane;
+        int outer = w.b, row = 0;
+        if (mine_i < w.i1) {
+          row = w.s.tile(mine_i) * kTileN;
+          if (p.c.pg.table) {
+            outer = __ldg(p.c.pg.table + static_cast<long>(w.b) * p.c.pg.table_stride + (row >> p.c.pg.page_shift));
+            row &= (1 << p.c.pg.page_shift) - 1;
+            if (static_cast<unsigned>(outer) >= static_cast<unsigned>(p.c.pg.n_pages)) {
+              report(p.c.error_flag, kStatusOutsideCache);
+              outer = 0;
+            }
+          }
+        }
+        const int cnt = min(32, w.i1 - base);
+        for (int k = 0; k < cnt; ++k, ++g) {
+          const int outer_k = __shfl_sync(0xffffffffu, outer, k), row_k = __shfl_sync(0xffffffffu, row, k);
+          const int s = g % kStages;
+          bool ok = true;
+          if (lane == 0) {
+            ok = mbar_wait(bar(BAR_EMPTY + s), ((g / kStages) & 1) ^ 1, abort_flag, p.c.error_flag, 31);
+            if (ok) {
+              // rows of the tile that some query row sees, in groups of 16
+              const int tpos = w.s.tile(base + k) * kTileN;
+              const int r0 = (tpos < w.s.ns ? 0 : max(0, w.s.lo - tpos)) & ~15;
+              const int r1 = (min(kTileN, w.s.end - tpos) + 15) & ~15;
+              const uint32_t full = bar(BAR_FULL + s);
+              const uint32_t dk = smem_base + s * kStageBytes, dv = dk + kTile;
+              const uint32_t dx = smem_base + kOffExp + s * 128;
+              const uint32_t rows = static_cast<uint32_t>(r1 - r0);
+              mbar_expect_tx(full, rows * 258);
+              if (rows == kTileN) {
+                tma_load_4d(dk, &map_k, full, 0, row_k, w.kvh, outer_k);
+                tma_load_4d(dv, &map_v, full, 0, row_k, w.kvh, outer_k);
+              } else {
+                for (int r = r0; r < r1; r += 16) {
+                  tma_load_4d(dk + r * 128, &map_k16, full, 0, row_k + r, w.kvh, outer_k);
+                  tma_load_4d(dv + r * 128, &map_v16, full, 0, row_k + r, w.kvh, outer_k);
+                }
+              }
+              const long xo = static_cast<long>(outer_k) * p.c.x_outer + w.kvh * p.c.x_head + row_k + r0;
+              bulk_load(dx + r0, p.c.kx + xo, rows, full);
+              bulk_load(dx + 64 + r0, p.c.vx + xo, rows, full);
+            }
+          }
+          if (!__shfl_sync(0xffffffffu, static_cast<int>(ok), 0)) return;
+        }
+      }
+    } while (w.next(p));
+    return;
+  }
+
+  if (warp == kConsumerWarps + 1) {
+    // ------------------------------------------------------------------ query rows
+    Walk w;
+    w.begin(p, b_first, off_first, x1 - x0);
+    unsigned char *q_s = smem + kOffQ;
+    float *qs = reinterpret_cast<float *>(smem + kOffQs);
+    int it = 0;
+    do {
+      const bool wait_ok = it == 0 || mbar_wait(bar(BAR_QFREE), (it - 1) & 1, abort_flag, p.c.error_flag, 32);
+      if (!__all_sync(0xffffffffu, wait_ok)) return;
+      const int nrows = w.s.nq * G;
+#pragma unroll
+      for (int it4 = 0; it4 < (WIDE ? 4 : 2); ++it4) {
+        const int rho = it4 * 4 + (lane >> 3), j = lane & 7; // eight lanes per row, 16 elements each
+        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
+        if (rho < nrows) {
+          const int tok = rho / G;
+          const T *src = static_cast<const T *>(p.q) + static_cast<long>(w.s.t0 + tok) * p.q_row + (w.kvh * G + rho - tok * G) * kHeadDim + 16 * j;
+          u0 = *reinterpret_cast<const uint4 *>(src);
+          u1 = *reinterpret_cast<const uint4 *>(src + 8);
+        }
+        float f[16];
+        const uint32_t ww[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 v = Elem<T>::unpack(ww[e]);
+          f[2 * e] = v.x, f[2 * e + 1] = v.y;
+          top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // the row's largest magnitude to 2^13 .. 2^14: an element keeps all its bits down to 2^-29 of it
+        int e = max(static_cast<int>(top >> 23) - 127, -100);
+        if (top >= 0x7f800000u) e = 13; // not finite: as it is
+        const float up = pow2i(13 - e);
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = Elem<__half>::pack(f[2 * i] * up, f[2 * i + 1] * up);
+        uint4 *dst = reinterpret_cast<uint4 *>(q_s + rho * 256 + j * 32);
+        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        if (j == 0) qs[rho] = p.scale_log2 * pow2i(e - 13);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(BAR_QREADY));
+      ++it;
+    } while (w.next(p));
+    return;
+  }
+
+  // -------------------------------------------------------------------- consumers
+  const int g0 = lane >> 2, cq = lane & 3;
+  const float kNegInf = -INFINITY, kNan = __int_as_float(0x7fc00000);
+  Walk w;
+  w.begin(p, b_first, off_first, x1 - x0);
+  uint32_t g = 0;
+  int it = 0;
+  bool ok = true; // a wait that gave up leaves a status; the warp goes on to the end without its tiles
+  do {
+    ok = ok && mbar_wait(bar(BAR_QREADY), it & 1, abort_flag, p.c.error_flag, 33);
+    // contraction order: k-step ks of this lane covers elements 32 cq + 4 ks + {0, 1} and + {2, 3}
+    uint32_t qa[8][4];
+    float qs0, qs1 = 0.f;
+    {
+      const uint4 *r0 = reinterpret_cast<const uint4 *>(smem + kOffQ + g0 * 256 + cq * 64);
+      const uint4 *r1 = reinterpret_cast<const uint4 *>(smem + kOffQ + (g0 + 8) * 256 + cq * 64);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint4 a = r0[x];
+        const uint4 b = WIDE ? r1[x] : make_uint4(0, 0, 0, 0);
+        qa[2 * x][0] = a.x, qa[2 * x][2] = a.y, qa[2 * x + 1][0] = a.z, qa[2 * x + 1][2] = a.w;
+        qa[2 * x][1] = b.x, qa[2 * x][3] = b.y, qa[2 * x + 1][1] = b.z, qa[2 * x + 1][3] = b.w;
+      }
+      const float *qs = reinterpret_cast<const float *>(smem + kOffQs);
+      qs0 = qs[g0];
+      if (WIDE) qs1 = qs[g0 + 8];
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(BAR_QFREE));
+
+    const int nrows = w.s.nq * G;
+    const int p0 = w.s.pos0 + g0 / G, p1 = w.s.pos0 + (g0 + 8) / G; // positions of this lane's rows
+    const int end0 = min(p0 + 1, w.s.end), end1 = min(p1 + 1, w.s.end);
+    const int lo0 = window_begin(p0, p.window), lo1 = window_begin(p1, p.window);
+    // every row sees all of a tile that ends before the first row's position and begins at or behind
+    // the last row's window, or lies among the first positions
+    const int all_end = min(w.s.pos0 + 1, w.s.end), all_lo = window_begin(w.s.pos0 + w.s.nq - 1, p.window);
+
+    float o[16][4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = kNegInf, m1 = kNegInf, l0 = 0.f, l1 = 0.f;
+
+    for (int i = w.i0; i < w.i1; ++i, ++g) {
+      const int s = g % kStages;
+      const int tpos = w.s.tile(i) * kTileN, col0 = tpos + warp * 16;
+      const bool some = col0 < w.s.end && (col0 + 15 >= w.s.lo || col0 < w.s.ns);
+      const bool all = tpos + kTileN <= all_end && (tpos >= all_lo || tpos + kTileN <= p.n_sink);
+      ok = ok && mbar_wait(bar(BAR_FULL + s), (g / kStages) & 1, abort_flag, p.c.error_flag, 34);
+      if (__all_sync(0xffffffffu, ok) && some) {
+        const uint32_t st_k = smem_base + s * kStageBytes, st_v = st_k + kTile;
+        const unsigned char *ex = smem + kOffExp + s * 128 + warp * 16;
+        float sc[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+          const uint32_t row = st_k + (warp * 16 + nt * 8 + g0) * 128;
+          uint32_t kw[8];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(kw[4 * x]), "=r"(kw[4 * x + 1]), "=r"(kw[4 * x + 2]), "=r"(kw[4 * x + 3])
+                         : "r"(row + (((2 * cq + x) ^ g0) << 4)));
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            mma_16816<__half>(sc[nt], qa[ks], cvt_e4m3x2_f16x2(kw[ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[ks] >> 16));
+        }
+        // exponents of this lane's four positions, two per n-tile
+        float vinv[4];
+        float tmax0 = kNegInf, tmax1 = kNegInf;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint32_t kx2 = *reinterpret_cast<const uint16_t *>(ex + nt * 8 + 2 * cq);
+          const uint32_t vx2 = *reinterpret_cast<const uint16_t *>(ex + 64 + nt * 8 + 2 * cq);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t kx = (kx2 >> (8 * e)) & 0xffu, vx = (vx2 >> (8 * e)) & 0xffu;
+            const float kf = (kx == kPoison || vx == kPoison) ? kNan : __uint_as_float(kx << 23);
+            const float ev = static_cast<float>(static_cast<int>(vx) - 127);
+            vinv[nt * 2 + e] = __uint_as_float((254u - min(vx, 253u)) << 23);
+            float t0 = fmaf(sc[nt][e], qs0 * kf, ev);
+            float t1 = WIDE ? fmaf(sc[nt][2 + e], qs1 * kf, ev) : 0.f;
+            if (!all) {
+              const int j = col0 + nt * 8 + 2 * cq + e;
+              if (!(j < end0 && (j >= lo0 || j < p.n_sink))) t0 = kNegInf;
+              if (WIDE && !(j < end1 && (j >= lo1 || j < p.n_sink))) t1 = kNegInf;
+            }
+            sc[nt][e] = t0;
+            tmax0 = fmaxf(tmax0, t0);
+            if (WIDE) {
+              sc[nt][2 + e] = t1;
+              tmax1 = fmaxf(tmax1, t1);
+            }
+          }
+        }
+        tmax0 = fmaxf(tmax0, __shfl_xor_sync(0xffffffffu, tmax0, 1));
+        tmax0 = fmaxf(tmax0, __shfl_xor_sync(0xffffffffu, tmax0, 2));
+        if (WIDE) {
+          tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 1));
+          tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 2));
+        }
+        const bool grow0 = tmax0 > m0 + kLazy, grow1 = WIDE && tmax1 > m1 + kLazy;
+        if (__any_sync(0xffffffffu, grow0 || grow1)) {
+          const float f0 = grow0 ? tc5::ex2(m0 - tmax0) : 1.f, f1 = grow1 ? tc5::ex2(m1 - tmax1) : 1.f;
+          if (grow0) m0 = tmax0;
+          if (grow1) m1 = tmax1;
+          l0 *= f0, l1 *= f1;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            o[x][0] *= f0, o[x][1] *= f0;
+            if (WIDE) o[x][2] *= f1, o[x][3] *= f1;
+          }
+        }
+        const float ms0 = m0 == kNegInf ? 0.f : m0, ms1 = m1 == kNegInf ? 0.f : m1; // nothing seen yet: P = 0
+        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const float a = tc5::ex2(sc[nt][0] - ms0), b = tc5::ex2(sc[nt][1] - ms0);
+          l0 = fmaf(a, vinv[2 * nt], l0);
+          l0 = fmaf(b, vinv[2 * nt + 1], l0);
+          pa[2 * nt] = Elem<__half>::pack(a, b);
+          if (WIDE) {
+            const float c2 = tc5::ex2(sc[nt][2] - ms1), d2 = tc5::ex2(sc[nt][3] - ms1);
+            l1 = fmaf(c2, vinv[2 * nt], l1);
+            l1 = fmaf(d2, vinv[2 * nt + 1], l1);
+            pa[2 * nt + 1] = Elem<__half>::pack(c2, d2);
+          }
+        }
+        // V: 16 bytes (elements 16 g0 ..) of rows 2 cq + {0, 1, 8, 9}
+        uint32_t vw[4][4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = 2 * cq + (x & 1) + (x >> 1) * 8; // row within the warp's 16
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(vw[x][0]), "=r"(vw[x][1]), "=r"(vw[x][2]), "=r"(vw[x][3])
+                       : "r"(st_v + (warp * 16 + r) * 128 + ((g0 ^ (r & 7)) << 4)));
+          if (!all) {
+            // a row nobody sees may hold anything: a zero weight must not meet a NaN code
+            const int j = col0 + r;
+            if (!(j < w.s.end && (j >= w.s.lo || j < w.s.ns))) vw[x][0] = vw[x][1] = vw[x][2] = vw[x][3] = 0u;
+          }
+        }
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const uint32_t lo2 = __byte_perm(vw[0][q4], vw[1][q4], hh ? 0x7362 : 0x5140);
+            const uint32_t hi2 = __byte_perm(vw[2][q4], vw[3][q4], hh ? 0x7362 : 0x5140);
+            const int x = 4 * q4 + 2 * hh;
+            mma_16816<__half>(o[x], pa, cvt_e4m3x2_f16x2(lo2 & 0xffffu), cvt_e4m3x2_f16x2(hi2 & 0xffffu));
+            mma_16816<__half>(o[x + 1], pa, cvt_e4m3x2_f16x2(lo2 >> 16), cvt_e4m3x2_f16x2(hi2 >> 16));
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(BAR_EMPTY + s));
+    }
+
+    // ---- the four warps' states of the piece -> its result.  Accumulator x of a lane holds elements
+    //      32 cq + x and 32 cq + 16 + x of its rows.
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (cq == 0) {
+      red_ml[(warp * 16 + g0) * 2] = m0;
+      red_ml[(warp * 16 + g0) * 2 + 1] = l0;
+      red_ml[(warp * 16 + g0 + 8) * 2] = m1;
+      red_ml[(warp * 16 + g0 + 8) * 2 + 1] = l1;
+    }
+    consumer_sync();
+    auto row_ml = [&](int row, float &M, float &L) {
+      M = kNegInf;
+#pragma unroll
+      for (int x = 0; x < kConsumerWarps; ++x) M = fmaxf(M, red_ml[(x * 16 + row) * 2]);
+      const float ms = M == kNegInf ? 0.f : M;
+      L = 0.f;
+#pragma unroll
+      for (int x = 0; x < kConsumerWarps; ++x) L += exp2f(red_ml[(x * 16 + row) * 2] - ms) * red_ml[(x * 16 + row) * 2 + 1];
+    };
+    const bool whole = w.i0 == 0 && w.i1 == w.s.n_tiles;
+    const int slot = 2 * c + (it == 0 ? 0 : 1);
+    float *buf = reinterpret_cast<float *>(smem + kOffCombine);
+#pragma unroll
+    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+      if (half * 8 < nrows) {
+        float M, L;
+        row_ml(g0 + 8 * half, M, L);
+        const float mw = half ? m1 : m0;
+        // L is NaN where a poisoned row was seen, and 0 where nothing was
+        const float f = L == 0.f ? 0.f : exp2f(mw - (M == kNegInf ? 0.f : M)) / L;
+#pragma unroll
+        for (int q8i = 0; q8i < 8; ++q8i) {
+          // chunk of four elements 32 cq + 4 q8i, its place turned by lane so that eight lanes hit eight banks
+          const int hi = q8i >> 2, x = (q8i & 3) * 4, e = 2 * half + hi;
+          const float4 v = make_float4(o[x][e] * f, o[x + 1][e] * f, o[x + 2][e] * f, o[x + 3][e] * f);
+          const int chunk = 8 * cq + (q8i ^ ((2 * cq + (g0 & 1)) & 7));
+          reinterpret_cast<float4 *>(buf)[(warp * 8 + g0) * 32 + chunk] = v;
+        }
+      }
+      consumer_sync();
+      const int rr = tid >> 4, rho = rr + 8 * half;
+      if (rho < nrows) {
+        const int tok = rho / G;
+        const long t = w.s.t0 + tok;
+        const int h = w.kvh * G + rho - tok * G;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int ch = (tid & 15) + 16 * k, cc = ch >> 3;
+          const int chunk = 8 * cc + ((ch & 7) ^ ((2 * cc + (rr & 1)) & 7));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int x = 0; x < kConsumerWarps; ++x) {
+            const float4 u = reinterpret_cast<const float4 *>(buf)[(x * 8 + rr) * 32 + chunk];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+          }
+          if (whole) {
+            uint2 u;
+            u.x = Elem<T>::pack(v.x, v.y);
+            u.y = Elem<T>::pack(v.z, v.w);
+            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + t * p.out_row + h * kHeadDim + 4 * ch) = u;
+          } else {
+            *reinterpret_cast<float4 *>(dp.ws.o + (static_cast<long>(slot) * dp.rows + rho) * kHeadDim + 4 * ch) = v;
+          }
+        }
+        if (!whole && (tid & 15) == 0) {
+          float M, L;
+          row_ml(rho, M, L);
+          dp.ws.lse[static_cast<long>(slot) * dp.rows + rho] = L == 0.f ? kNegInf : (M == kNegInf ? 0.f : M) + log2f(L);
+        }
+      }
+      consumer_sync(); // the buffer and red_ml may be written again
+    }
+    if (w.i0 == 0 && tid == 0) {
+      // this CTA holds the run's first tile: it says which CTAs hold the others
+      const long first = x1 - w.left; // the piece's place on the line
+      const int last = share_of(W, n, first + w.s.n_tiles - 1);
+      RunInfo r;
+      r.c0 = c, r.c1 = last, r.slot0 = slot, r.pad = 0;
+      dp.ws.info[static_cast<long>(w.b) * kvH + w.kvh] = r;
+    }
+    ++it;
+  } while (w.next(p));
+}
+
+// Merges the pieces of the runs that were cut, and zeroes the rows that see nothing.  Grid: (sequence and
+// KV head, row); warp i folds pieces i, i + 4, ... in order, and the warps' results are joined in order.
+template <typename T> __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8DecodeParams dp) {
+  using namespace q8d;
+  __shared__ float4 xo[4][32];
+  __shared__ float2 xml[4];
+  const Q8AttnParams &p = dp.a;
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+  const int kvH = p.c.n_kv_heads, G = p.group;
+  const int b = blockIdx.x / kvH, kvh = blockIdx.x - b * kvH, rho = blockIdx.y;
+  const Seq s = seq_of(p, b);
+  if (rho >= s.nq * G) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s.n_tiles > 0) {
+    const RunInfo info = dp.ws.info[blockIdx.x];
+    if (info.c1 <= info.c0) return;      // the run was not cut
+    const int parts = info.c1 - info.c0 + 1;
+    float M = -INFINITY, W = 0.f;
+    for (int x = warp; x < parts; x += 4) {
+      const long row = static_cast<long>(x == 0 ? info.slot0 : 2 * (info.c0 + x)) * dp.rows + rho;
+      const float l = dp.ws.lse[row];
+      const float4 v = *reinterpret_cast<const float4 *>(dp.ws.o + row * kHeadDim + lane * 4);
+      if (l == -INFINITY) continue;
+      const float mn = fmaxf(M, l);
+      const float fa = exp2f(M - mn), fb = exp2f(l - mn);
+      W = W * fa + fb;
+      acc.x = acc.x * fa + fb * v.x, acc.y = acc.y * fa + fb * v.y, acc.z = acc.z * fa + fb * v.z, acc.w = acc.w * fa + fb * v.w;
+      M = mn;
+    }
+    xo[warp][lane] = acc;
+    if (lane == 0) xml[warp] = make_float2(M, W);
+    __syncthreads();
+    if (warp != 0) return;
+    const float Mx = fmaxf(fmaxf(xml[0].x, xml[1].x), fmaxf(xml[2].x, xml[3].x));
+    float Wt = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = 0; x < 4; ++x) {
+      const float2 ml = xml[x];
+      if (ml.y == 0.f) continue;         // no piece, or none that sees anything
+      const float f = exp2f(ml.x - (Mx == -INFINITY ? 0.f : Mx));
+      const float4 u = xo[x][lane];
+      Wt += f * ml.y;
+      acc.x += f * u.x, acc.y += f * u.y, acc.z += f * u.z, acc.w += f * u.w;
+    }
+    if (Wt != 0.f) acc.x /= Wt, acc.y /= Wt, acc.z /= Wt, acc.w /= Wt; // NaN divides too
+  } else if (warp != 0) {
+    return;
+  }
+  const int tok = rho / G;
+  uint2 u;
+  u.x = Elem<T>::pack(acc.x, acc.y);
+  u.y = Elem<T>::pack(acc.z, acc.w);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + static_cast<long>(s.t0 + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = u;
+}
+
+namespace {
+
+template <typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// the shared-memory opt-in is a property of (function, device): set on the first launch per device
+template <typename T, bool WIDE> cudaError_t opt_in() {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    e = cudaFuncSetAttribute(attn_q8_decode_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, q8d::kSmemTotal);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return e;
+}
+
+template <typename T, bool WIDE>
+cudaError_t launch_typed(const Q8DecodeParams &dp, int n_ctas, const CUtensorMap *m, cudaStream_t stream, int *launches) {
+  cudaError_t e = opt_in<T, WIDE>();
+  if (e != cudaSuccess) return e;
+  e = launch_dependent(attn_q8_decode_kernel<T, WIDE>, dim3(n_ctas), q8d::kThreads, q8d::kSmemTotal, stream, m[0], m[1], m[2], m[3], dp);
+  if (e != cudaSuccess) return e;
+  *launches = 1;
+  e = launch_dependent(attn_q8_merge_kernel<T>, dim3(dp.a.c.batch * dp.a.c.n_kv_heads, dp.rows), 128, 0, stream, dp);
+  if (e != cudaSuccess) return e;
+  *launches = 2;
+  return cudaGetLastError();
+}
+
+int cta_count(int batch, int n_kv_heads, int max_kv_len) {
+  const long tiles = static_cast<long>(batch) * n_kv_heads * ((static_cast<long>(max_kv_len) + q8d::kTileN - 1) / q8d::kTileN);
+  return static_cast<int>(tiles < q8d::kMaxCtas ? tiles : q8d::kMaxCtas);
+}
+
+} // namespace
+
+size_t attn_q8_decode_ws_bytes(int batch, int n_kv_heads, int rows, int max_kv_len) {
+  const size_t slots = 2 * static_cast<size_t>(cta_count(batch, n_kv_heads, max_kv_len));
+  const size_t parts = (slots * rows * (kHeadDim + 1) * sizeof(float) + 15) / 16 * 16;
+  return parts + static_cast<size_t>(batch) * n_kv_heads * sizeof(q8d::RunInfo);
+}
+
+cudaError_t launch_attn_q8_decode(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches) {
+  *launches = 0;
+  const Q8Cache &c = p.c;
+  Q8DecodeParams dp{};
+  dp.a = p;
+  dp.rows = p.max_new * p.group;
+  dp.min_tiles = 1;
+  const int n_ctas = cta_count(c.batch, c.n_kv_heads, p.max_kv_len);
+  const size_t slots = 2 * static_cast<size_t>(n_ctas);
+  dp.ws.o = static_cast<float *>(p.ws);
+  dp.ws.lse = dp.ws.o + slots * dp.rows * kHeadDim;
+  dp.ws.info = reinterpret_cast<q8d::RunInfo *>(static_cast<char *>(p.ws) + (slots * dp.rows * (kHeadDim + 1) * sizeof(float) + 15) / 16 * 16);
+  // (d, position, kv head, sequence), or (d, position in page, kv head, page)
+  const uint64_t rows = c.pg.table ? 1ull << c.pg.page_shift : static_cast<uint64_t>(c.max_pos);
+  const uint64_t outers = c.pg.table ? static_cast<uint64_t>(c.pg.n_pages) : static_cast<uint64_t>(c.batch);
+  CUtensorMap m[4];
+  const void *base[2] = {c.k, c.v};
+  for (int i = 0; i < 4; ++i)
+    if (!make_tensor_map_u8(&m[i], true, base[i & 1], rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, i < 2 ? 64 : 16))
+      return cudaErrorNotSupported;
+  const bool wide = dp.rows > 8;
+  if (bf16)
+    return wide ? launch_typed<__nv_bfloat16, true>(dp, n_ctas, m, stream, launches) : launch_typed<__nv_bfloat16, false>(dp, n_ctas, m, stream, launches);
+  return wide ? launch_typed<__half, true>(dp, n_ctas, m, stream, launches) : launch_typed<__half, false>(dp, n_ctas, m, stream, launches);
+}
+
+} // namespace b200attn

@@ -467,28 +467,33 @@ int *error_word() {
   return words[dev];
 }
 
-// 4-D map over (d, dim1, dim2, dim3) with a box of 64 x box1 x box2 x 1 elements
-bool make_tensor_map_4d_impl(CUtensorMap *map, bool bf16, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1, long s2,
+// 4-D map over (d, dim1, dim2, dim3).  16-bit elements: box of 64 x box1 x box2 x 1, 128-byte swizzle;
+// 8-bit codes (elem == kMapU8, kMapU8Swizzled): box of 128 x box1 x box2 x 1, dense or with that swizzle.
+bool make_tensor_map_4d_impl(CUtensorMap *map, uint32_t elem, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1, long s2,
               long s3, uint32_t box1, uint32_t box2) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  auto fix = [](long s) { return static_cast<cuuint64_t>(s > 0 ? s : 128) * 2; }; // bytes; unit extents may carry stride 0
+  const bool u8 = elem >= kMapU8;
+  const cuuint64_t eb = u8 ? 1 : 2;
+  auto fix = [eb](long s) { return static_cast<cuuint64_t>(s > 0 ? s : 128) * eb; }; // bytes; unit extents may carry stride 0
   cuuint64_t dims[4] = {128, n1, n2, n3};
   cuuint64_t strides[3] = {fix(s1), fix(s2), fix(s3)};
-  cuuint32_t box[4] = {64, box1, box2, 1};
+  cuuint32_t box[4] = {u8 ? 128u : 64u, box1, box2, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < 3; ++i)
     if (strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
-  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                  const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType type = u8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                      : elem ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = fn(map, type, 4, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  elem == kMapU8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
 
 } // namespace tc5
 
-bool make_tensor_map_4d(CUtensorMap *map, bool bf16, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1,
-                        long s2, long s3, uint32_t box1, uint32_t box2) {
+static bool cached_tensor_map(CUtensorMap *map, uint32_t elem, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1,
+                              long s2, long s3, uint32_t box1, uint32_t box2) {
   // the encoding depends on nothing but these arguments: keep the most recent ones per thread
   constexpr int kCached = 32;
   struct Entry {
@@ -500,19 +505,29 @@ bool make_tensor_map_4d(CUtensorMap *map, bool bf16, const void *base, uint64_t 
   thread_local int next = 0;
   TensorMapKey key{};
   key.base = base, key.n1 = n1, key.n2 = n2, key.n3 = n3, key.s1 = s1, key.s2 = s2, key.s3 = s3;
-  key.box1 = box1, key.box2 = box2, key.bf16 = bf16 ? 1u : 0u;
+  key.box1 = box1, key.box2 = box2, key.elem = elem;
   for (int i = 0; i < kCached; ++i) {
     if (cache[i].used && memcmp(&cache[i].key, &key, sizeof key) == 0) {
       *map = cache[i].map;
       return true;
     }
   }
-  if (!tc5::make_tensor_map_4d_impl(map, bf16, base, n1, n2, n3, s1, s2, s3, box1, box2)) return false;
+  if (!tc5::make_tensor_map_4d_impl(map, elem, base, n1, n2, n3, s1, s2, s3, box1, box2)) return false;
   cache[next].key = key;
   cache[next].map = *map;
   cache[next].used = true;
   next = (next + 1) % kCached;
   return true;
+}
+
+bool make_tensor_map_4d(CUtensorMap *map, bool bf16, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1,
+                        long s2, long s3, uint32_t box1, uint32_t box2) {
+  return cached_tensor_map(map, bf16 ? 1u : 0u, base, n1, n2, n3, s1, s2, s3, box1, box2);
+}
+
+bool make_tensor_map_u8(CUtensorMap *map, bool swizzle, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1, long s2,
+                        long s3, uint32_t box1) {
+  return cached_tensor_map(map, swizzle ? kMapU8Swizzled : kMapU8, base, n1, n2, n3, s1, s2, s3, box1, 1);
 }
 
 int *kernel_error_word_dev() {

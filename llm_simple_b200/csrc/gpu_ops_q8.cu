@@ -124,6 +124,15 @@ int check_attention(const gpu_attn_desc *d, const void *out, const void *q, int 
   return GPU_OPS_OK;
 }
 
+int check_workspace(const void *workspace, size_t given, size_t need) {
+  if (need && (!workspace || given < need)) return fail(GPU_OPS_E_WORKSPACE, "workspace of %zu bytes given, %zu needed", given, need);
+  if (!aligned16(workspace)) return fail(GPU_OPS_E_INVALID, "workspace must be 16-byte aligned");
+  return GPU_OPS_OK;
+}
+
+// Query rows of a KV head that the decode kernel takes at once.
+bool few_rows(int max_new, int group) { return static_cast<long>(max_new) * group <= 16; }
+
 float scale_log2_of_128() { return (1.0f / sqrtf(128.0f)) * 1.4426950408889634f; }
 
 } // namespace
@@ -182,9 +191,8 @@ int gpu_kv_read_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, c
 }
 
 size_t gpu_attn_decode_q8_workspace_bytes(const gpu_attn_desc *desc, int max_kv_len) {
-  (void)desc;
-  (void)max_kv_len;
-  return 0;
+  if (!desc || desc->batch <= 0 || desc->n_kv_heads <= 0 || desc->n_heads < desc->n_kv_heads || max_kv_len <= 0) return 0;
+  return attn_q8_decode_ws_bytes(desc->batch, desc->n_kv_heads, desc->n_heads / desc->n_kv_heads, max_kv_len);
 }
 
 int gpu_attn_decode_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *out, const void *q,
@@ -197,8 +205,8 @@ int gpu_attn_decode_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *page
   if (!kv_len_dev) return fail(GPU_OPS_E_INVALID, "null kv_len");
   if (int rc = check_row("q_seq_stride", desc->q_seq_stride, desc->n_heads)) return rc;
   if (int rc = check_row("out_seq_stride", desc->out_seq_stride, desc->n_heads)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, gpu_attn_decode_q8_workspace_bytes(desc, max_kv_len))) return rc;
   if (int rc = status_word(&p.c)) return rc;
-  (void)workspace_bytes;
   p.kv_len = kv_len_dev;
   p.out = out;
   p.q = q;
@@ -213,17 +221,19 @@ int gpu_attn_decode_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *page
   p.scale_log2 = scale_log2_of_128();
   p.ws = workspace;
   int launches = 0;
-  cudaError_t e = launch_attn_q8(p, desc->dtype == GPU_DT_BFLOAT16, static_cast<cudaStream_t>(stream), &launches);
+  cudaError_t e = launch_attn_q8_decode(p, desc->dtype == GPU_DT_BFLOAT16, static_cast<cudaStream_t>(stream), &launches);
   add_launch_count(launches);
+  if (e == cudaErrorNotSupported) return fail(GPU_OPS_E_UNSUPPORTED, "the cache strides cannot be described by a TMA tensor map");
   if (e != cudaSuccess) return cuda_fail(e, "8-bit decode attention launch");
   return GPU_OPS_OK;
 }
 
 size_t gpu_attn_chunk_q8_workspace_bytes(const gpu_attn_desc *desc, int total_tokens, int max_new, int max_kv_len) {
-  (void)desc;
-  (void)total_tokens;
-  (void)max_new;
-  (void)max_kv_len;
+  if (!desc || desc->batch <= 0 || desc->n_kv_heads <= 0 || desc->n_heads < desc->n_kv_heads || total_tokens <= 0 || max_new <= 0 ||
+      max_kv_len <= 0)
+    return 0;
+  if (few_rows(max_new, desc->n_heads / desc->n_kv_heads))
+    return attn_q8_decode_ws_bytes(desc->batch, desc->n_kv_heads, max_new * (desc->n_heads / desc->n_kv_heads), max_kv_len);
   return 0;
 }
 
@@ -241,8 +251,9 @@ int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages
   if (int rc = check_row("q_tok_stride", desc->q_tok_stride, desc->n_heads)) return rc;
   if (int rc = check_row("out_tok_stride", desc->out_tok_stride, desc->n_heads)) return rc;
   if (total_tokens == 0) return GPU_OPS_OK;
+  if (int rc = check_workspace(workspace, workspace_bytes, gpu_attn_chunk_q8_workspace_bytes(desc, total_tokens, max_new, max_kv_len)))
+    return rc;
   if (int rc = status_word(&p.c)) return rc;
-  (void)workspace_bytes;
   p.out = out;
   p.q = q;
   p.q_row = desc->q_tok_stride;
@@ -256,8 +267,11 @@ int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages
   p.scale_log2 = scale_log2_of_128();
   p.ws = workspace;
   int launches = 0;
-  cudaError_t e = launch_attn_q8(p, desc->dtype == GPU_DT_BFLOAT16, static_cast<cudaStream_t>(stream), &launches);
+  const bool bf16 = desc->dtype == GPU_DT_BFLOAT16;
+  cudaError_t e = few_rows(max_new, p.group) ? launch_attn_q8_decode(p, bf16, static_cast<cudaStream_t>(stream), &launches)
+                                             : launch_attn_q8(p, bf16, static_cast<cudaStream_t>(stream), &launches);
   add_launch_count(launches);
+  if (e == cudaErrorNotSupported) return fail(GPU_OPS_E_UNSUPPORTED, "the cache strides cannot be described by a TMA tensor map");
   if (e != cudaSuccess) return cuda_fail(e, "8-bit chunk attention launch");
   return GPU_OPS_OK;
 }

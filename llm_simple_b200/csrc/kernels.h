@@ -223,8 +223,9 @@ struct TensorMapKey {
   const void *base;
   uint64_t n1, n2, n3;
   long s1, s2, s3;
-  uint32_t box1, box2, bf16, pad; // no padding bytes: compared with memcmp
+  uint32_t box1, box2, elem, pad; // elem: 0 fp16, 1 bf16, or one of the below; no padding bytes: compared with memcmp
 };
+constexpr uint32_t kMapU8 = 2, kMapU8Swizzled = 3;
 // Non-zero once a bounded wait inside a kernel on the current device has given up.
 int attn_tc5_error_status();
 void attn_clear_error_status();
@@ -286,6 +287,9 @@ struct Q8AttnParams {
   float scale_log2;
   void *ws;
 };
+// Up to 16 query rows per (sequence, KV head): the decode form, and chunks with max_new * group <= 16.
+cudaError_t launch_attn_q8_decode(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches);
+size_t attn_q8_decode_ws_bytes(int batch, int n_kv_heads, int rows, int max_kv_len);
 cudaError_t launch_attn_q8(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches);
 
 // ---- cross-device (O, LSE) exchange + merge over peer memory ------------------

@@ -20,6 +20,9 @@ namespace b200attn {
 // cannot be encoded (strides not multiples of 16 bytes, extents too large).
 bool make_tensor_map_4d(CUtensorMap *map, bool bf16, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1,
                         long s2, long s3, uint32_t box1, uint32_t box2);
+// The same over 8-bit codes: strides in bytes, box 128 x box1 x 1 x 1 bytes, with the 128-byte swizzle or dense.
+bool make_tensor_map_u8(CUtensorMap *map, bool swizzle, const void *base, uint64_t n1, uint64_t n2, uint64_t n3, long s1, long s2,
+                        long s3, uint32_t box1);
 
 namespace tma {
 
@@ -83,6 +86,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+
+// Untiled copy global -> shared; both addresses and the size are multiples of 16 bytes.  No multicast.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
 }
 
 } // namespace tma

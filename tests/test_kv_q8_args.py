@@ -144,6 +144,18 @@ def test_attention(call):
         _refused(_decode(_desc(), None, _kv(), lens=None), E_INVALID, "kv_len")
 
 
+def test_workspace():
+    need = ops.gpu_attn_decode_q8_workspace_bytes(_desc(), 256)
+    assert need > 0
+    _refused(_decode(_desc(), None, _kv(), ws=None), E_WORKSPACE, "workspace")
+    _refused(_decode(_desc(), None, _kv(), n=need - 1), E_WORKSPACE, "%d needed" % need)
+    _refused(_decode(_desc(), None, _kv(), ws=A + 8), E_INVALID, "workspace must be")
+    need = ops.gpu_attn_chunk_q8_workspace_bytes(_desc(), 5, 3, 256)
+    _refused(_chunk(_desc(), None, _kv(), n=need - 1), E_WORKSPACE, "%d needed" % need)
+    for bad in ((None, 256), (_desc(), 0)):
+        assert ops.lib().gpu_attn_decode_q8_workspace_bytes(_r(bad[0]), bad[1]) == 0
+
+
 def test_struct_matches_the_header_layout():
     assert ctypes.sizeof(ops.KvQ8) == 4 * 8 + 2 * 8 + 2 * 4
     assert ops.KvQ8.exp_outer_stride.offset == 32 and ops.KvQ8.max_pos.offset == 48
