@@ -17,7 +17,7 @@ OBJ = os.path.join(HERE, "csrc", "_obj")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_SOURCES = ["rope_append.cu", "attn_mma.cu", "attn_tc5.cu", "attn_tc5p.cu", "gpu_ops.cu", "decode_noalloc.cu", "xchg_merge.cu",
-                "attn_decode_tma.cu", "kv_q8.cu", "attn_q8.cu", "attn_q8_decode.cu", "gpu_ops_q8.cu"]
+                "attn_decode_tma.cu", "kv_q8.cu", "attn_q8_decode.cu", "attn_q8_chunk.cu", "gpu_ops_q8.cu"]
 CXX_SOURCES = ["decode_plan.cpp", "host/device_gpu.cpp", "host/attention_layer_gpu.cpp", "host/host_abi.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"),

@@ -1,0 +1,851 @@
+// Causal attention of ragged chunks of new tokens over the 8-bit KV cache, on the 5th-generation
+// tensor cores.
+//
+// A block is up to 2 x 128 query rows of one KV head and one sequence: 128 / group tokens times the
+// group's heads in each of two tiles A and B, so that every cache tile, once in shared memory, serves
+// all heads that share it.  A block walks the tiles of 128 positions that its rows see.  The walks of
+// all blocks are laid end to end and every CTA (one per SM) takes an equal, contiguous share of that
+// line; where the line is cut inside a block, the pieces leave normalised partials and log-sum-exps
+// that a second, dependent launch merges in a fixed order.  The lengths are read on the device.
+//
+// 16 warps in four groups:
+//   warp 0       TMA producer: e4m3 tiles of K and V in boxes of 64 positions, with their exponents
+//   warp 1       MMA issuer: S_X = Q_X K^T, then O_X += P_X V with P from tensor memory
+//   warps 4-11   softmax of tile A (4-7) and B (8-11), one thread per query row; they also bring the
+//                rows of Q in and the results out
+//   warps 12-15  converters: e4m3 -> fp16 operand tiles
+// All products run on fp16.  e4m3 codes are exact in it, and Q is scaled by a power of two per row.
+// The row exponents of a tile are taken relative to the largest one of the tile, r = max e: the
+// converters scale row j by 2^(7 + e_j - r), which is exact for all codes as long as e_j is within 22
+// of r (a row 2^22 below its tile's largest loses bits that lie 2^-41 below that row).  Then
+//     t = S 2^(r_k - 7) scale log2(e) + (r_v - 7),  P = 2^(t - max t),  O += P V',  l += 2^(7 - r_v) sum P
+// where r_k, r_v are constants of the tile: the softmax costs what it costs over 16-bit caches.
+// P is rounded to fp16 (at most 2^8: O is rescaled only when the maximum grew by more than that).
+// A position outside every row's view is converted to zeros whatever its bytes are; a position whose
+// exponent says "not finite" becomes a NaN row of K' and zeros in V', so that exactly the rows that
+// see it turn NaN.
+//
+// Bound by the tensor pipe and, equally, the exponentials: 128 x 128 x 16 products take 64 cycles, so
+// a tile of 128 positions against 256 rows takes 2048 cycles, as do its 32768 exponentials at 16 a
+// cycle.
+#include "q8.cuh"
+#include "tc5.cuh"
+#include "tma.cuh"
+
+namespace b200attn {
+
+namespace q8c {
+
+using namespace q8;
+using namespace tma;
+using namespace tc5;
+
+constexpr int kThreads = 512;
+constexpr int kBN = 128;
+constexpr uint32_t kHalfTile = 128 * 128;            // [128 rows][64 fp16], swizzled
+constexpr uint32_t kTileBytes = 2 * kHalfTile;
+constexpr uint32_t kRawBytes = 128 * 128;            // e4m3 tile
+constexpr uint32_t kSmemQ = 0;                       // Q_A, Q_B
+constexpr uint32_t kSmemK = kSmemQ + 2 * kTileBytes; // two stages
+constexpr uint32_t kSmemV = kSmemK + 2 * kTileBytes;
+constexpr uint32_t kSmemRaw = kSmemV + 2 * kTileBytes; // K, V
+constexpr uint32_t kSmemExp = kSmemRaw + 2 * kRawBytes; // K [128], V [128]
+constexpr uint32_t kSmemRef = kSmemExp + 256;        // [4][r_k, r_v]
+constexpr uint32_t kSmemScan = kSmemRef + 32;        // 16 + 8 ints
+constexpr uint32_t kSmemBar = kSmemScan + 96;
+constexpr uint32_t kSmemTotal = kSmemBar + 256;
+static_assert(kSmemTotal <= 232448, "shared memory of one CTA");
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256;
+constexpr float kLazy = 8.0f;
+constexpr int kMaxCtas = 148;
+constexpr int kMaxBatch = 16000;                     // prefix sums of the batch lie in the Q tiles while a CTA finds its share
+
+enum { BAR_RAWFULL = 0, BAR_RAWEMPTY = 2, BAR_KFULL = 4, BAR_KEMPTY = 6, BAR_VFULL = 8, BAR_VEMPTY = 10, BAR_QFULL = 12, BAR_SFULL = 14,
+       BAR_PHALF = 16, BAR_PREADY = 18, BAR_ODONE = 20, BAR_REF = 22, BAR_QTAKEN = 26, BAR_COUNT = 28 };
+static_assert(BAR_COUNT * 8 + 8 <= 256, "barrier block");
+
+using Block = Span<kBN>;
+
+struct Head { // 16 bytes, at the front of the workspace
+  int n_blocks, pad[3];
+};
+// What a block's pieces left: the CTAs c0 .. c1 (c1 < c0: no row sees anything), the slot of the first
+// (of the others it is 2 c), and the block's rows.
+struct RunInfo {
+  int c0, c1, slot0, t0, nq, pad[3];
+};
+
+} // namespace q8c
+
+struct Q8ChunkParams {
+  Q8AttnParams a;
+  int tile_tokens;      // tokens per tile of 128 rows: 128 / group
+  int min_tiles, max_blocks;
+  q8c::Head *head;
+  q8c::RunInfo *info;   // [blocks][kv heads]
+  float *o, *lse;       // [slot][2 * tile_tokens * group][128], and without the 128
+};
+
+namespace q8c {
+
+// Block blk of sequence b.
+__device__ __forceinline__ Block block_of(const Q8ChunkParams &cp, int b, int blk) {
+  const Q8AttnParams &p = cp.a;
+  int t0, nq, pos0, limit;
+  chunk_rows(p, b, false, t0, nq, pos0, limit);
+  const int first = blk * 2 * cp.tile_tokens;
+  Block s;
+  s.t0 = t0 + first;
+  s.nq = min(2 * cp.tile_tokens, nq - first);
+  s.pos0 = pos0 + first;
+  s.cover(p, limit);
+  return s;
+}
+__device__ __forceinline__ int blocks_of(const Q8ChunkParams &cp, int b) {
+  int t0, nq, pos0, limit;
+  chunk_rows(cp.a, b, blockIdx.x == 0, t0, nq, pos0, limit);
+  return (nq + 2 * cp.tile_tokens - 1) / (2 * cp.tile_tokens);
+}
+
+struct Walk {
+  int b, blk, n_blk, kvh, i0, i1;
+  long left;
+  Block s;
+  __device__ __forceinline__ void begin(const Q8ChunkParams &cp, int b_, int blk_, long offset, long tiles) {
+    b = b_, blk = blk_;
+    n_blk = blocks_of(cp, b);
+    s = block_of(cp, b, blk);
+    kvh = static_cast<int>(offset / s.n_tiles);
+    i0 = static_cast<int>(offset - static_cast<long>(kvh) * s.n_tiles);
+    left = tiles;
+    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), i0 + left));
+  }
+  __device__ __forceinline__ bool next(const Q8ChunkParams &cp) {
+    left -= i1 - i0;
+    if (left <= 0) return false;
+    if (++kvh == cp.a.c.n_kv_heads) {
+      kvh = 0;
+      do {
+        if (++blk >= n_blk) {
+          blk = 0;
+          do {
+            if (++b >= cp.a.c.batch) return false;
+            n_blk = blocks_of(cp, b);
+          } while (n_blk == 0);
+        }
+        s = block_of(cp, b, blk);
+      } while (s.n_tiles == 0);
+    }
+    i0 = 0;
+    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), left));
+    return true;
+  }
+};
+
+// The rows of tile X of a block: their first and last positions, and which cache tiles they see.
+struct Half {
+  int first, last, n_tok;    // positions; number of tokens (0: the tile is empty)
+  int lo_first, lo_last;     // first window positions of the first and of the last row
+  __device__ __forceinline__ void of(const Q8ChunkParams &cp, const Block &s, int x) {
+    n_tok = max(0, min(cp.tile_tokens, s.nq - x * cp.tile_tokens));
+    first = s.pos0 + x * cp.tile_tokens;
+    last = first + n_tok - 1;
+    lo_first = window_begin(first, cp.a.window);
+    lo_last = window_begin(last, cp.a.window);
+  }
+  __device__ __forceinline__ bool sees(const Q8ChunkParams &cp, int col0) const { // some row, something of the tile
+    return n_tok > 0 && col0 <= last && (col0 + kBN > lo_first || col0 < cp.a.n_sink);
+  }
+  __device__ __forceinline__ bool sees_all(const Q8ChunkParams &cp, const Block &s, int col0) const { // every row, all of it
+    return col0 + kBN <= min(first + 1, s.end) && (col0 >= lo_last || col0 + kBN <= cp.a.n_sink);
+  }
+};
+
+__device__ __forceinline__ int block_scan(int mine, int *scratch, int warp, int lane, int &total) { // exclusive; all threads
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  int before = incl - mine;
+  total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int v = scratch[w];
+    if (w < warp) before += v;
+    total += v;
+  }
+  __syncthreads();
+  return before;
+}
+
+} // namespace q8c
+
+template <typename T>
+__global__ void __launch_bounds__(q8c::kThreads, 1)
+attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8ChunkParams cp) {
+  using namespace q8c;
+  const Q8AttnParams &p = cp.a;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t smem_base = smem_u32(smem);
+  int *scan = reinterpret_cast<int *>(smem + kSmemScan);
+  volatile int *refs = reinterpret_cast<volatile int *>(smem + kSmemRef);
+  volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + kSmemBar + BAR_COUNT * 8);
+  volatile uint32_t *abort_flag = tmem_slot + 1;
+  auto bar = [&](int i) { return smem_base + kSmemBar + 8u * i; };
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.group, kvH = p.c.n_kv_heads, tok2 = 2 * cp.tile_tokens;
+  int *err = p.c.error_flag;
+
+  cudaTriggerProgrammaticLaunchCompletion();
+  if (tid == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(BAR_RAWFULL + s), 1);
+      mbar_init(bar(BAR_RAWEMPTY + s), 4);
+      mbar_init(bar(BAR_KFULL + s), 4);
+      mbar_init(bar(BAR_KEMPTY + s), 1);
+      mbar_init(bar(BAR_VFULL + s), 4);
+      mbar_init(bar(BAR_VEMPTY + s), 1);
+      mbar_init(bar(BAR_QFULL + s), 128);
+      mbar_init(bar(BAR_SFULL + s), 1);
+      mbar_init(bar(BAR_PHALF + s), 128);
+      mbar_init(bar(BAR_PREADY + s), 128);
+      mbar_init(bar(BAR_ODONE + s), 1);
+      mbar_init(bar(BAR_QTAKEN + s), 1);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(bar(BAR_REF + s), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  cudaGridDependencySynchronize();
+
+  // ---- this CTA's share.  Blocks before each sequence (in the Q tiles), then tiles before each block.
+  int *prefix = reinterpret_cast<int *>(smem + kSmemQ);
+  int n_blocks;
+  {
+    const int per = (p.c.batch + kThreads - 1) / kThreads;
+    const int lo = min(p.c.batch, tid * per), hi = min(p.c.batch, lo + per);
+    int mine = 0;
+    for (int b = lo; b < hi; ++b) mine += blocks_of(cp, b);
+    int at = block_scan(mine, scan, warp, lane, n_blocks);
+    for (int b = lo; b < hi; ++b) {
+      prefix[b] = at;
+      at += blocks_of(cp, b);
+    }
+    if (tid == 0) prefix[p.c.batch] = n_blocks;
+    __syncthreads();
+  }
+  if (n_blocks > cp.max_blocks) { // tok_start decreases somewhere: the rows overlap
+    if (tid == 0) report(err, kStatusOutsideCache);
+    n_blocks = 0;
+  }
+  const int per = (n_blocks + kThreads - 1) / kThreads;
+  const int u_lo = min(n_blocks, tid * per), u_hi = min(n_blocks, u_lo + per);
+  int b_lo = 0;
+  if (u_lo < u_hi) { // the sequence of block u_lo: the last one with prefix <= u_lo
+    int len = p.c.batch;
+    while (len > 1) {
+      const int half = len / 2;
+      if (prefix[b_lo + half] <= u_lo) b_lo += half;
+      len -= half;
+    }
+  }
+  int mine = 0;
+  for (int u = u_lo, b = b_lo; u < u_hi; ++u) {
+    while (u >= prefix[b + 1]) ++b;
+    mine += block_of(cp, b, u - prefix[b]).n_tiles;
+  }
+  int total;
+  const int before = block_scan(mine, scan, warp, lane, total);
+  const long W = static_cast<long>(total) * kvH;
+  const int n = static_cast<int>(min(static_cast<long>(gridDim.x), (W + cp.min_tiles - 1) / cp.min_tiles));
+  const int c = blockIdx.x;
+  const long x0 = c < n ? share_begin(W, n, c) : -1, x1 = c < n ? share_begin(W, n, c + 1) : -1;
+  if (c == 0 && tid == 0) cp.head->n_blocks = n_blocks;
+  {
+    long at = static_cast<long>(before) * kvH;
+    for (int u = u_lo, b = b_lo; u < u_hi; ++u) {
+      while (u >= prefix[b + 1]) ++b;
+      const Block s = block_of(cp, b, u - prefix[b]);
+      const long run = static_cast<long>(s.n_tiles) * kvH;
+      if (x0 >= at && x0 < at + run) {
+        scan[16] = b;
+        scan[17] = u - prefix[b];
+        scan[18] = static_cast<int>(x0 - at);
+      }
+      if (u % gridDim.x == c) { // the CTAs share the writing of the merge's records
+        for (int h = 0; h < kvH; ++h) {
+          RunInfo r{};
+          r.c1 = -1;
+          if (s.n_tiles > 0) {
+            const long first = at + static_cast<long>(h) * s.n_tiles;
+            r.c0 = share_of(W, n, first);
+            r.c1 = share_of(W, n, first + s.n_tiles - 1);
+            r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) == first ? 0 : 1);
+          }
+          r.t0 = s.t0;
+          r.nq = s.nq;
+          cp.info[static_cast<long>(u) * kvH + h] = r;
+        }
+      }
+      at += run;
+    }
+  }
+  if ((smem_base & 1023u) != 0 && tid == 0) report(err, 30);
+  __syncthreads();
+  if (c >= n || (smem_base & 1023u) != 0) return;
+  const int b_first = scan[16], blk_first = scan[17], off_first = scan[18];
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t *>(tmem_slot))), "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads(); // also: the prefix sums in the Q tiles are done with
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    reg_dec<64>();
+    Walk w;
+    if (warp == 0) {
+      // ---------------------------------------------------------- TMA producer
+      w.begin(cp, b_first, blk_first, off_first, x1 - x0);
+      uint32_t g = 0;
+      bool ok = true;
+      do {
+        for (int base = w.i0; base < w.i1 && ok; base += 16) {
+          // lanes 2 k, 2 k + 1: the two halves of the k-th tile from here: page, row in it, and whether anyone sees it
+          int outer = w.b, row = 0;
+          bool on = false;
+          if (base + (lane >> 1) < w.i1) {
+            row = w.s.tile(base + (lane >> 1)) * kBN + 64 * (lane & 1);
+            on = row < w.s.end && (row + 64 > w.s.lo || row < w.s.ns);
+            if (on && p.c.pg.table) {
+              outer = __ldg(p.c.pg.table + static_cast<long>(w.b) * p.c.pg.table_stride + (row >> p.c.pg.page_shift));
+              row &= (1 << p.c.pg.page_shift) - 1;
+              if (static_cast<unsigned>(outer) >= static_cast<unsigned>(p.c.pg.n_pages)) {
+                report(err, kStatusOutsideCache);
+                outer = 0;
+              }
+            }
+          }
+          const int cnt = min(16, w.i1 - base);
+          for (int k = 0; k < cnt && ok; ++k, ++g) {
+            int o[2], r[2];
+            bool live[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              o[h] = __shfl_sync(0xffffffffu, outer, 2 * k + h);
+              r[h] = __shfl_sync(0xffffffffu, row, 2 * k + h);
+              live[h] = __shfl_sync(0xffffffffu, static_cast<int>(on), 2 * k + h) != 0;
+            }
+            if (lane == 0) {
+#pragma unroll
+              for (int kv = 0; kv < 2; ++kv) {
+                ok = ok && mbar_wait(bar(BAR_RAWEMPTY + kv), (g & 1) ^ 1, abort_flag, err, 1);
+                if (!ok) break;
+                const uint32_t full = bar(BAR_RAWFULL + kv);
+                uint32_t bytes = 0, xb[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  // exponent rows of a flat cache end at max_pos rounded up to 16
+                  xb[h] = p.c.pg.table ? 64u : static_cast<uint32_t>(min(64, ((p.c.max_pos + 15) & ~15) - r[h]));
+                  if (live[h]) bytes += 64 * 128 + (kv == 0 ? 2 * xb[h] : 0);
+                }
+                mbar_expect_tx(full, bytes);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  if (!live[h]) continue;
+                  tma_load_4d(smem_base + kSmemRaw + kv * kRawBytes + h * 64 * 128, kv ? &map_v : &map_k, full, 0, r[h], w.kvh, o[h]);
+                  if (kv == 0) { // the exponents of V come along: the softmax needs their largest with K
+                    const long xo = static_cast<long>(o[h]) * p.c.x_outer + w.kvh * p.c.x_head + r[h];
+                    bulk_load(smem_base + kSmemExp + 64 * h, p.c.kx + xo, xb[h], full);
+                    bulk_load(smem_base + kSmemExp + 128 + 64 * h, p.c.vx + xo, xb[h], full);
+                  }
+                }
+              }
+            }
+            ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+          }
+        }
+      } while (ok && w.next(cp));
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      w.begin(cp, b_first, blk_first, off_first, x1 - x0);
+      constexpr uint32_t idesc_qk = instr_desc(0u, 0), idesc_pv = instr_desc(0u, 1);
+      const uint32_t dq0 = smem_desc_lo(smem_base + kSmemQ, 16);
+      const uint32_t dk0 = smem_desc_lo(smem_base + kSmemK, 16);
+      const uint32_t dv0 = smem_desc_lo(smem_base + kSmemV, kHalfTile);
+      constexpr uint32_t kTileStep = kTileBytes >> 4, kHalfStep = kHalfTile >> 4;
+      uint32_t g = 0;                 // tiles of the share so far
+      uint32_t cnt[2] = {0, 0};       // P.V products issued for A and B
+      int piece = 0;
+      bool ok = true;
+      auto issue_qk = [&](int x, uint32_t gt) {
+        const uint32_t d = tmem + kColS + 128 * x, dq = dq0 + x * kTileStep, dk = dk0 + (gt & 1) * kTileStep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t ko = (k >> 2) * kHalfStep + (k & 3) * 2;
+          tc_mma_ss(d, dq + ko, dk + ko, kDescHi, idesc_qk, k > 0);
+        }
+        tc_commit(bar(BAR_SFULL + x));
+      };
+      auto issue_pv = [&](int x, uint32_t gt, bool first) -> bool {
+        if (!mbar_wait(bar(BAR_PHALF + x), cnt[x] & 1, abort_flag, err, 10)) return false;
+        if (!mbar_wait(bar(BAR_VFULL + (gt & 1)), (gt >> 1) & 1, abort_flag, err, 6)) return false;
+        tc_fence_after();
+        const uint32_t pcol = tmem + kColS + 128 * x, ocol = tmem + kColO + 128 * x;
+        const uint32_t dv = dv0 + (gt & 1) * kTileStep;
+        const uint32_t acc0 = first ? 0u : 1u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_ts(ocol, pcol + 8 * k, dv + k * (2048 >> 4), kDescHi, idesc_pv, k > 0 ? 1u : acc0);
+        if (!mbar_wait(bar(BAR_PREADY + x), cnt[x] & 1, abort_flag, err, 5)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 4; k < 8; ++k) tc_mma_ts(ocol, pcol + 8 * k, dv + k * (2048 >> 4), kDescHi, idesc_pv, 1u);
+        tc_commit(bar(BAR_ODONE + x));
+        ++cnt[x];
+        return true;
+      };
+      do {
+        Half hx[2];
+        hx[0].of(cp, w.s, 0);
+        hx[1].of(cp, w.s, 1);
+        bool begun[2] = {false, false};
+        // K of the piece's first tile, and the rows of Q (their writers have also taken the previous results out)
+        ok = mbar_wait(bar(BAR_KFULL + (g & 1)), (g >> 1) & 1, abort_flag, err, 4);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          ok = ok && mbar_wait(bar(BAR_QFULL + x), piece & 1, abort_flag, err, 3);
+          if (!ok) break;
+          mbar_arrive(bar(BAR_QTAKEN + x));
+          tc_fence_after();
+          if (hx[x].sees(cp, w.s.tile(w.i0) * kBN)) issue_qk(x, g);
+        }
+        if (ok) tc_commit(bar(BAR_KEMPTY + (g & 1)));
+        for (int i = w.i0; ok && i < w.i1; ++i, ++g) {
+          const int col0 = w.s.tile(i) * kBN;
+          const bool more = i + 1 < w.i1;
+          const int col1 = more ? w.s.tile(i + 1) * kBN : 0;
+          if (more) ok = mbar_wait(bar(BAR_KFULL + ((g + 1) & 1)), ((g + 1) >> 1) & 1, abort_flag, err, 4);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ok && hx[x].sees(cp, col0)) {
+              ok = issue_pv(x, g, !begun[x]);
+              begun[x] = true;
+            }
+            if (ok && more && hx[x].sees(cp, col1)) {
+              tc_fence_after();
+              issue_qk(x, g + 1);
+            }
+          }
+          if (ok) {
+            ok = mbar_wait(bar(BAR_VFULL + (g & 1)), (g >> 1) & 1, abort_flag, err, 6); // a stage is freed only after it was filled
+            tc_commit(bar(BAR_VEMPTY + (g & 1)));
+            if (more) tc_commit(bar(BAR_KEMPTY + ((g + 1) & 1)));
+          }
+        }
+        ++piece;
+      } while (ok && w.next(cp));
+    }
+  } else if (warp < 12) {
+    reg_inc<184>();
+    // ------------------------------------------------------------ softmax, Q and results of tile X
+    const int x = (warp >> 2) - 1, quad = warp & 3;
+    const int r = quad * 32 + lane;              // row of the tile
+    const int tok = r / G, hd = r - tok * G;     // its token and head of the group
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t scol = tmem + lane_addr + kColS + 128 * x, ocol = tmem + lane_addr + kColO + 128 * x;
+    Walk w;
+    w.begin(cp, b_first, blk_first, off_first, x1 - x0);
+    uint32_t g = 0, cnt = 0;
+    int piece = 0;
+    bool ok = true;
+    do {
+      Half hx;
+      hx.of(cp, w.s, x);
+      const bool live = tok < hx.n_tok;          // tok < tile_tokens for every row that exists
+      const long t = static_cast<long>(w.s.t0) + x * cp.tile_tokens + tok;
+      // a tile that sees nothing of a piece must not run more than one piece ahead of the MMA warp
+      if (piece > 0 && !__all_sync(0xffffffffu, mbar_wait(bar(BAR_QTAKEN + x), (piece - 1) & 1, abort_flag, err, 13))) break;
+      // ---- the row of Q, scaled to fp16: its largest magnitude to 2^13 .. 2^14
+      float rowc;
+      {
+        uint4 u[16];
+        uint32_t top = 0;
+        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + t * p.q_row + (w.kvh * G + hd) * kHeadDim);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) u[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t *wd = reinterpret_cast<const uint32_t *>(&u[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = Elem<T>::unpack(wd[e]);
+            top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+          }
+        }
+        int e = max(static_cast<int>(top >> 23) - 127, -100);
+        if (top >= 0x7f800000u) e = 13;          // not finite: as it is
+        const float up = pow2i(13 - e);
+        rowc = p.scale_log2 * pow2i(e - 13);
+        const uint32_t dst = smem_base + kSmemQ + x * kTileBytes + r * 128;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          uint32_t *wd = reinterpret_cast<uint32_t *>(&u[i]);
+#pragma unroll
+          for (int e2 = 0; e2 < 4; ++e2) {
+            const float2 v = Elem<T>::unpack(wd[e2]);
+            wd[e2] = Elem<__half>::pack(v.x * up, v.y * up);
+          }
+          const uint32_t chunk = static_cast<uint32_t>(i & 7) ^ static_cast<uint32_t>(r & 7);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kHalfTile + (chunk << 4)), "r"(u[i].x), "r"(u[i].y),
+                       "r"(u[i].z), "r"(u[i].w)
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      mbar_arrive(bar(BAR_QFULL + x));
+
+      const int pos = hx.first + tok;
+      const int vend = live ? min(pos + 1, w.s.end) : 0, wlo = window_begin(pos, p.window);
+      float m_ref = -INFINITY, l = 0.f;
+      bool begun = false;
+      for (int i = w.i0; i < w.i1; ++i, ++g) {
+        const int col0 = w.s.tile(i) * kBN;
+        if (!hx.sees(cp, col0)) continue;
+        ok = ok && mbar_wait(bar(BAR_SFULL + x), cnt & 1, abort_flag, err, 7);
+        ok = ok && mbar_wait(bar(BAR_REF + (g & 3)), (g >> 2) & 1, abort_flag, err, 12); // complete by now: K was converted before S
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int rk = refs[2 * (g & 3)], rv = refs[2 * (g & 3) + 1];
+        const float a = fmaxf(rowc * pow2i(rk - 7), 1.2e-38f), off = static_cast<float>(rv - 7);
+        uint32_t su[128];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) tc_ld32(scol + 32 * q4, su + 32 * q4);
+        tc_wait_ld();
+        if (!hx.sees_all(cp, w.s, col0)) {
+          const int ve = vend - col0, wl = wlo - col0, sk = p.n_sink - col0;
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (!(j < ve && (j >= wl || j < sk))) su[j] = 0xff800000u; // -inf
+        }
+        float mxa[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mxa[j] = fmaxf(__uint_as_float(su[j]), __uint_as_float(su[8 + j]));
+#pragma unroll
+        for (int j = 16; j < 128; j += 16) {
+#pragma unroll
+          for (int q8i = 0; q8i < 8; ++q8i) mxa[q8i] = max3(mxa[q8i], __uint_as_float(su[j + q8i]), __uint_as_float(su[j + 8 + q8i]));
+        }
+        const float top = fmaxf(max3(mxa[0], mxa[1], mxa[2]), fmaxf(max3(mxa[3], mxa[4], mxa[5]), fmaxf(mxa[6], mxa[7])));
+        const float mx = fmaf(top, a, off);
+        const bool grow = mx > m_ref + kLazy;
+        if (__any_sync(0xffffffffu, grow) && begun) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(BAR_ODONE + x), (cnt - 1) & 1, abort_flag, err, 8))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float f = grow ? ex2(m_ref - mx) : 1.f;
+          l *= f;
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint32_t o[32];
+            tc_ld32(ocol + 32 * q4, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tc_st32(ocol + 32 * q4, o);
+          }
+          tc_wait_st();
+        }
+        if (grow) m_ref = mx;
+        begun = true;
+        const float nm = off - (m_ref == -INFINITY ? 0.f : m_ref); // nothing seen yet: P = 0
+        uint32_t pk[64];
+        uint64_t sums[2] = {0ull, 0ull};
+        const uint64_t a2 = pack2(a, a), nm2 = pack2(nm, nm);
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          const uint64_t y2 = fma2(pack2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), a2, nm2);
+          float y0, y1;
+          unpack2(y2, y0, y1);
+          const float e0 = ex2(y0), e1 = ex2(y1);
+          sums[j & 1] = add2(sums[j & 1], pack2(e0, e1));
+          pk[j] = Elem<__half>::pack(e0, e1);
+          if (j == 31) {
+            tc_st32(scol, pk);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(BAR_PHALF + x));
+          }
+        }
+        {
+          float s0, s1, s2, s3;
+          unpack2(sums[0], s0, s1);
+          unpack2(sums[1], s2, s3);
+          l = fmaf((s0 + s1) + (s2 + s3), pow2i(7 - rv), l);
+        }
+        tc_st32(scol + 32, pk + 32);
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(BAR_PREADY + x));
+        ++cnt;
+      }
+      if (!ok) break;
+      // ---- the piece's result
+      if (begun && !__all_sync(0xffffffffu, mbar_wait(bar(BAR_ODONE + x), (cnt - 1) & 1, abort_flag, err, 9))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool whole = w.i0 == 0 && w.i1 == w.s.n_tiles;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
+      const long slot_row = static_cast<long>(2 * c + (piece == 0 ? 0 : 1)) * (tok2 * G) + (x * cp.tile_tokens + tok) * G + hd;
+      T *dst = static_cast<T *>(p.out) + t * p.out_row + (w.kvh * G + hd) * kHeadDim;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        uint32_t o[32];
+        if (begun) {
+          tc_ld32(ocol + 32 * q4, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        if (live && whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint4 v;
+            v.x = Elem<T>::pack(__uint_as_float(o[8 * j]) * inv, __uint_as_float(o[8 * j + 1]) * inv);
+            v.y = Elem<T>::pack(__uint_as_float(o[8 * j + 2]) * inv, __uint_as_float(o[8 * j + 3]) * inv);
+            v.z = Elem<T>::pack(__uint_as_float(o[8 * j + 4]) * inv, __uint_as_float(o[8 * j + 5]) * inv);
+            v.w = Elem<T>::pack(__uint_as_float(o[8 * j + 6]) * inv, __uint_as_float(o[8 * j + 7]) * inv);
+            reinterpret_cast<uint4 *>(dst)[4 * q4 + j] = v;
+          }
+        } else if (live) {
+          float4 *part = reinterpret_cast<float4 *>(cp.o + slot_row * kHeadDim);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            part[8 * q4 + j] = make_float4(__uint_as_float(o[4 * j]) * inv, __uint_as_float(o[4 * j + 1]) * inv,
+                                           __uint_as_float(o[4 * j + 2]) * inv, __uint_as_float(o[4 * j + 3]) * inv);
+        }
+        __syncwarp(); // tcgen05.ld takes the whole warp
+      }
+      if (live && !whole) cp.lse[slot_row] = l == 0.f ? -INFINITY : (m_ref == -INFINITY ? 0.f : m_ref) + log2f(l);
+      ++piece;
+    } while (w.next(cp));
+  } else {
+    reg_dec<80>();
+    // ------------------------------------------------------------ converters: 32 rows of every tile per warp
+    const int cw = warp - 12;
+    Walk w;
+    w.begin(cp, b_first, blk_first, off_first, x1 - x0);
+    uint32_t g = 0;
+    bool ok = true;
+    // rows 32 cw .. 32 cw + 31 of the raw tile -> fp16 operand tile; `f`: this lane's row's factor, two fp16 (0: zeros)
+    auto convert = [&](uint32_t raw, uint32_t dst, uint32_t f) {
+#pragma unroll 4
+      for (int it = 0; it < 8; ++it) {
+        const int rl = it * 4 + (lane >> 3), row = 32 * cw + rl, ch = lane & 7; // 16 codes: elements 16 ch ..
+        const uint32_t fr = __shfl_sync(0xffffffffu, f, rl);
+        uint32_t wv[4], h[8];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(wv[0]), "=r"(wv[1]), "=r"(wv[2]), "=r"(wv[3]) : "r"(raw + row * 128 + ch * 16));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t v = hmul2(cvt_e4m3x2_f16x2((wv[e >> 1] >> (16 * (e & 1))) & 0xffffu), fr);
+          h[e] = fr ? v : 0u;
+        }
+        // two 16-byte chunks of the row's half tile; lanes of the two halves write them in opposite order
+        // (the halves lie 16 KB apart, in the same banks)
+        const uint32_t base = dst + (ch >> 2) * kHalfTile + row * 128, c0 = 2 * (ch & 3), flip = ch >> 2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t q = k ^ flip;
+          const uint32_t at = base + (((c0 + q) ^ (row & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q ? h[4] : h[0]), "r"(q ? h[5] : h[1]), "r"(q ? h[6] : h[2]),
+                       "r"(q ? h[7] : h[3])
+                       : "memory");
+        }
+      }
+    };
+    // 2^(7 - d) as two fp16; d: how far the row's exponent lies below the tile's largest
+    auto factor = [](int d) -> uint32_t {
+      const uint32_t h = d <= 21 ? static_cast<uint32_t>(15 + 7 - d) << 10 : d <= 31 ? 1u << (31 - d) : 0u;
+      return h | (h << 16);
+    };
+    do {
+      for (int i = w.i0; ok && i < w.i1; ++i, ++g) {
+        const int col0 = w.s.tile(i) * kBN;
+        const uint32_t ph = g & 1, s = g & 1, sph = (g >> 1) & 1;
+        ok = mbar_wait(bar(BAR_RAWFULL + 0), ph, abort_flag, err, 20);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        // the largest exponents among the rows that someone sees (every warp for itself: 4 rows a lane)
+        const uint32_t kx4 = *reinterpret_cast<const uint32_t *>(smem + kSmemExp + 4 * lane);
+        const uint32_t vx4 = *reinterpret_cast<const uint32_t *>(smem + kSmemExp + 128 + 4 * lane);
+        auto seen = [&](int j) { return j < w.s.end && (j >= w.s.lo || j < w.s.ns); };
+        int rk = 0, rv = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int kx = (kx4 >> (8 * e)) & 0xff, vx = (vx4 >> (8 * e)) & 0xff;
+          if (seen(col0 + 4 * lane + e) && kx != kPoison && vx != kPoison) rk = max(rk, kx), rv = max(rv, vx);
+        }
+        rk = __reduce_max_sync(0xffffffffu, rk);
+        rv = __reduce_max_sync(0xffffffffu, rv);
+        const int row = 32 * cw + lane;
+        const int kx = smem[kSmemExp + row], vx = smem[kSmemExp + 128 + row];
+        const bool vis = seen(col0 + row), poison = kx == kPoison || vx == kPoison;
+        const uint32_t fk = !vis ? 0u : poison ? 0x7e007e00u : factor(rk - kx);
+        const uint32_t fv = !vis || poison ? 0u : factor(rv - vx);
+        ok = mbar_wait(bar(BAR_KEMPTY + s), sph ^ 1, abort_flag, err, 21);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        convert(smem_base + kSmemRaw, smem_base + kSmemK + s * kTileBytes, fk);
+        if (cw == 0 && lane == 0) {
+          refs[2 * (g & 3)] = rk - 127;
+          refs[2 * (g & 3) + 1] = rv - 127;
+          mbar_arrive(bar(BAR_REF + (g & 3)));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(BAR_KFULL + s));
+          mbar_arrive(bar(BAR_RAWEMPTY + 0));
+        }
+        ok = mbar_wait(bar(BAR_RAWFULL + 1), ph, abort_flag, err, 22) && mbar_wait(bar(BAR_VEMPTY + s), sph ^ 1, abort_flag, err, 23);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        convert(smem_base + kSmemRaw + kRawBytes, smem_base + kSmemV + s * kTileBytes, fv);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(BAR_VFULL + s));
+          mbar_arrive(bar(BAR_RAWEMPTY + 1));
+        }
+      }
+    } while (__all_sync(0xffffffffu, ok) && w.next(cp));
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Merges the pieces of the blocks that were cut, and zeroes the rows that see nothing.  Grid: (block and
+// KV head, groups of 32 rows); a warp takes four rows and folds their pieces in order.
+template <typename T> __global__ void __launch_bounds__(256) attn_q8_chunk_merge_kernel(const Q8ChunkParams cp) {
+  using namespace q8c;
+  const Q8AttnParams &p = cp.a;
+  cudaTriggerProgrammaticLaunchCompletion();
+  cudaGridDependencySynchronize();
+  const int kvH = p.c.n_kv_heads, G = p.group;
+  const int u = blockIdx.x / kvH, kvh = blockIdx.x - u * kvH;
+  if (u >= cp.head->n_blocks) return;
+  const RunInfo info = cp.info[blockIdx.x];
+  if (info.c1 == info.c0) return; // one CTA did the whole block
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int block_rows = 2 * cp.tile_tokens * G;
+  for (int k = 0; k < 4; ++k) {
+    const int rho = blockIdx.y * 32 + warp * 4 + k;
+    if (rho >= info.nq * G) return;
+    float M = -INFINITY, Wt = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = info.c0; c <= info.c1; ++c) {
+      const long row = static_cast<long>(c == info.c0 ? info.slot0 : 2 * c) * block_rows + rho;
+      const float l = cp.lse[row];
+      const float4 v = *reinterpret_cast<const float4 *>(cp.o + row * kHeadDim + lane * 4);
+      if (l == -INFINITY) continue;
+      const float mn = fmaxf(M, l);
+      const float fa = exp2f(M - mn), fb = exp2f(l - mn);
+      Wt = Wt * fa + fb;
+      acc.x = acc.x * fa + fb * v.x, acc.y = acc.y * fa + fb * v.y, acc.z = acc.z * fa + fb * v.z, acc.w = acc.w * fa + fb * v.w;
+      M = mn;
+    }
+    if (Wt != 0.f) acc.x /= Wt, acc.y /= Wt, acc.z /= Wt, acc.w /= Wt;
+    const int tok = rho / G;
+    uint2 o;
+    o.x = Elem<T>::pack(acc.x, acc.y);
+    o.y = Elem<T>::pack(acc.z, acc.w);
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (static_cast<long>(info.t0) + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = o;
+  }
+}
+
+namespace {
+
+// Blocks a batch can have at most, and CTAs to launch.
+long block_bound(int batch, int group, int total) {
+  const int tok2 = 2 * (128 / group);
+  return total / tok2 + (batch < total ? batch : total);
+}
+int chunk_ctas(int batch, int n_kv_heads, int group, int total, int max_kv_len) {
+  const long tiles = block_bound(batch, group, total) * n_kv_heads * ((static_cast<long>(max_kv_len) + q8c::kBN - 1) / q8c::kBN);
+  return static_cast<int>(tiles < q8c::kMaxCtas ? tiles : q8c::kMaxCtas);
+}
+
+template <typename T> cudaError_t launch_typed(const Q8ChunkParams &cp, const CUtensorMap &mk, const CUtensorMap &mv, int n_ctas, long blocks, cudaStream_t stream, int *launches) {
+  // the shared-memory opt-in is a property of (function, device): set on the first launch per device
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    e = cudaFuncSetAttribute(attn_q8_chunk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, q8c::kSmemTotal);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  e = launch_dependent(attn_q8_chunk_kernel<T>, dim3(n_ctas), q8c::kThreads, q8c::kSmemTotal, stream, mk, mv, cp);
+  if (e != cudaSuccess) return e;
+  *launches = 1;
+  const int rows = 2 * cp.tile_tokens * cp.a.group;
+  e = launch_dependent(attn_q8_chunk_merge_kernel<T>, dim3(static_cast<unsigned>(blocks * cp.a.c.n_kv_heads), (rows + 31) / 32), 256, 0, stream, cp);
+  if (e != cudaSuccess) return e;
+  *launches = 2;
+  return cudaGetLastError();
+}
+
+} // namespace
+
+size_t attn_q8_chunk_ws_bytes(int batch, int n_kv_heads, int group, int total, int max_kv_len) {
+  const size_t rows = 2 * static_cast<size_t>(chunk_ctas(batch, n_kv_heads, group, total, max_kv_len)) * (2 * (128 / group) * group);
+  return sizeof(q8c::Head) + static_cast<size_t>(block_bound(batch, group, total)) * n_kv_heads * sizeof(q8c::RunInfo) +
+         rows * (kHeadDim + 1) * sizeof(float);
+}
+
+cudaError_t launch_attn_q8_chunk(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches) {
+  *launches = 0;
+  const Q8Cache &c = p.c;
+  if (c.batch > q8c::kMaxBatch) return cudaErrorNotSupported;
+  Q8ChunkParams cp{};
+  cp.a = p;
+  cp.tile_tokens = 128 / p.group;
+  cp.min_tiles = 1;
+  cp.max_blocks = static_cast<int>(block_bound(c.batch, p.group, p.r.total));
+  const int n_ctas = chunk_ctas(c.batch, c.n_kv_heads, p.group, p.r.total, p.max_kv_len);
+  const long blocks = block_bound(c.batch, p.group, p.r.total);
+  char *ws = static_cast<char *>(p.ws);
+  cp.head = reinterpret_cast<q8c::Head *>(ws);
+  cp.info = reinterpret_cast<q8c::RunInfo *>(ws + sizeof(q8c::Head));
+  cp.o = reinterpret_cast<float *>(ws + sizeof(q8c::Head) + static_cast<size_t>(blocks) * c.n_kv_heads * sizeof(q8c::RunInfo));
+  cp.lse = cp.o + 2 * static_cast<size_t>(n_ctas) * (2 * cp.tile_tokens * p.group) * kHeadDim;
+  const uint64_t rows = c.pg.table ? 1ull << c.pg.page_shift : static_cast<uint64_t>(c.max_pos);
+  const uint64_t outers = c.pg.table ? static_cast<uint64_t>(c.pg.n_pages) : static_cast<uint64_t>(c.batch);
+  CUtensorMap mk, mv;
+  if (!make_tensor_map_u8(&mk, false, c.k, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64) ||
+      !make_tensor_map_u8(&mv, false, c.v, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64))
+    return cudaErrorNotSupported;
+  return bf16 ? launch_typed<__nv_bfloat16>(cp, mk, mv, n_ctas, blocks, stream, launches)
+              : launch_typed<__half>(cp, mk, mv, n_ctas, blocks, stream, launches);
+}
+
+} // namespace b200attn

@@ -58,20 +58,11 @@ static_assert(BAR_COUNT * 8 + 8 <= 128, "barrier block");
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumerThreads) : "memory"); }
 
-// One sequence's rows and the tiles they see.
-struct Seq {
-  int t0, nq;          // its first row and number of rows
-  int pos0;            // position of the first row
-  int end;             // one past the last visible position
-  int lo;              // first window position of the first row
-  int ns;              // first positions visible besides the window
-  int ns_tiles, w0, n_tiles; // tiles 0 .. ns_tiles - 1, then w0, w0 + 1, ...
-  __device__ __forceinline__ int tile(int i) const { return i < ns_tiles ? i : w0 + i - ns_tiles; }
-};
+using Seq = Span<kTileN>;
 
 __device__ __forceinline__ Seq seq_of(const Q8AttnParams &p, int b) {
   Seq s;
-  const int limit = min(p.max_kv_len, p.c.max_pos);
+  int limit = min(p.max_kv_len, p.c.max_pos);
   if (p.kv_len) {
     const int len = __ldg(p.kv_len + b);
     if (len > limit) report(p.c.error_flag, kStatusLengthBeyondBound);
@@ -79,33 +70,12 @@ __device__ __forceinline__ Seq seq_of(const Q8AttnParams &p, int b) {
     s.nq = 1;
     s.pos0 = min(len, limit) - 1;
   } else {
-    const int a = min(max(__ldg(p.r.tok_start + b), 0), p.r.total), e = min(max(__ldg(p.r.tok_start + b + 1), a), p.r.total);
-    s.t0 = a;
-    s.nq = e - a;
-    s.pos0 = __ldg(p.r.start_pos + b);
-    if (s.nq > p.max_new) {
-      report(p.c.error_flag, kStatusLengthBeyondBound);
-      s.nq = p.max_new;
-    }
-    if (s.nq > 0) {
-      const long last = static_cast<long>(s.pos0) + s.nq - 1;
-      if (s.pos0 < 0 || last >= p.c.max_pos) report(p.c.error_flag, kStatusOutsideCache);
-      else if (last >= limit) report(p.c.error_flag, kStatusLengthBeyondBound);
-      s.pos0 = max(s.pos0, -32);
-    }
+    chunk_rows(p, b, true, s.t0, s.nq, s.pos0, limit);
+    s.nq = min(s.nq, p.max_new);
   }
-  s.end = s.nq > 0 ? max(0, static_cast<int>(min(static_cast<long>(s.pos0) + s.nq, static_cast<long>(limit)))) : 0;
-  s.lo = min(window_begin(s.pos0, p.window), s.end);
-  s.ns = min(p.n_sink, s.lo);
-  s.ns_tiles = (s.ns + kTileN - 1) / kTileN;
-  s.w0 = max(s.lo / kTileN, s.ns_tiles);
-  s.n_tiles = s.end > 0 ? s.ns_tiles + max(0, (s.end + kTileN - 1) / kTileN - s.w0) : 0;
+  s.cover(p, limit);
   return s;
 }
-
-// Share c of a line of W tiles cut for n CTAs, and the CTA that owns tile x.
-__device__ __forceinline__ long share_begin(long W, int n, int c) { return static_cast<long>(c) * W / n; }
-__device__ __forceinline__ int share_of(long W, int n, long x) { return static_cast<int>(((x + 1) * n - 1) / W); }
 
 // The pieces of one CTA's share, in order.
 struct Walk {
@@ -640,21 +610,6 @@ template <typename T> __global__ void __launch_bounds__(128) attn_q8_merge_kerne
 }
 
 namespace {
-
-template <typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // the shared-memory opt-in is a property of (function, device): set on the first launch per device
 template <typename T, bool WIDE> cudaError_t opt_in() {

@@ -234,7 +234,7 @@ size_t gpu_attn_chunk_q8_workspace_bytes(const gpu_attn_desc *desc, int total_to
     return 0;
   if (few_rows(max_new, desc->n_heads / desc->n_kv_heads))
     return attn_q8_decode_ws_bytes(desc->batch, desc->n_kv_heads, max_new * (desc->n_heads / desc->n_kv_heads), max_kv_len);
-  return 0;
+  return attn_q8_chunk_ws_bytes(desc->batch, desc->n_kv_heads, desc->n_heads / desc->n_kv_heads, total_tokens, max_kv_len);
 }
 
 int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *out, const void *q,
@@ -269,7 +269,7 @@ int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages
   int launches = 0;
   const bool bf16 = desc->dtype == GPU_DT_BFLOAT16;
   cudaError_t e = few_rows(max_new, p.group) ? launch_attn_q8_decode(p, bf16, static_cast<cudaStream_t>(stream), &launches)
-                                             : launch_attn_q8(p, bf16, static_cast<cudaStream_t>(stream), &launches);
+                                             : launch_attn_q8_chunk(p, bf16, static_cast<cudaStream_t>(stream), &launches);
   add_launch_count(launches);
   if (e == cudaErrorNotSupported) return fail(GPU_OPS_E_UNSUPPORTED, "the cache strides cannot be described by a TMA tensor map");
   if (e != cudaSuccess) return cuda_fail(e, "8-bit chunk attention launch");

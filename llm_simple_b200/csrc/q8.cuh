@@ -55,6 +55,11 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2_f16x2(uint32_t u) {
   asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(u));
   return r;
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // Two fp32 values -> two e4m3 codes (a in the low byte), to nearest even.
 __device__ __forceinline__ uint32_t cvt_f32_e4m3x2(float a, float b) {
   uint16_t r;
@@ -74,5 +79,59 @@ __device__ __forceinline__ int row_exp(float amax) {
 // One query row's visible positions: [0, min(sink, lo)) and [lo, pos].
 __device__ __forceinline__ int window_begin(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
+// The tiles of TILE positions that a run of consecutive rows sees: those of the first positions, 0 ..
+// ns_tiles - 1, and those from the first row's window to the last row, w0, w0 + 1, ...
+template <int TILE> struct Span {
+  int t0, nq;          // the first row and the number of rows
+  int pos0;            // position of the first row
+  int end;             // one past the last visible position
+  int lo;              // first window position of the first row
+  int ns;              // first positions visible besides the window
+  int ns_tiles, w0, n_tiles;
+  __device__ __forceinline__ int tile(int i) const { return i < ns_tiles ? i : w0 + i - ns_tiles; }
+  __device__ __forceinline__ void cover(const Q8AttnParams &p, int limit) { // from t0, nq, pos0
+    end = nq > 0 ? max(0, static_cast<int>(min(static_cast<long>(pos0) + nq, static_cast<long>(limit)))) : 0;
+    lo = min(window_begin(pos0, p.window), end);
+    ns = min(p.n_sink, lo);
+    ns_tiles = (ns + TILE - 1) / TILE;
+    w0 = max(lo / TILE, ns_tiles);
+    n_tiles = end > 0 ? ns_tiles + max(0, (end + TILE - 1) / TILE - w0) : 0;
+  }
+};
+
+// Rows of sequence b in the chunk form; `complain`: report bounds that do not hold.
+__device__ __forceinline__ void chunk_rows(const Q8AttnParams &p, int b, bool complain, int &t0, int &nq, int &pos0, int &limit) {
+  limit = min(p.max_kv_len, p.c.max_pos);
+  const int a = min(max(__ldg(p.r.tok_start + b), 0), p.r.total), e = min(max(__ldg(p.r.tok_start + b + 1), a), p.r.total);
+  t0 = a;
+  nq = e - a;
+  pos0 = __ldg(p.r.start_pos + b);
+  if (nq > 0 && complain) {
+    const long last = static_cast<long>(pos0) + nq - 1;
+    if (pos0 < 0 || last >= p.c.max_pos) report(p.c.error_flag, kStatusOutsideCache);
+    else if (last >= limit || nq > p.max_new) report(p.c.error_flag, kStatusLengthBeyondBound);
+  }
+}
+
+// Share c of a line of W tiles cut for n CTAs, and the CTA that owns tile x.
+__device__ __forceinline__ long share_begin(long W, int n, int c) { return static_cast<long>(c) * W / n; }
+__device__ __forceinline__ int share_of(long W, int n, long x) { return static_cast<int>(((x + 1) * n - 1) / W); }
+
 } // namespace q8
+
+template <typename... Args>
+inline cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 } // namespace b200attn

@@ -434,6 +434,21 @@ def test_chunk_few_rows_and_long_caches(ops, new, start, window, sink):
     assert torch.equal(out, _chunk(ops, c, q, new, start, window, sink))
 
 
+@pytest.mark.parametrize("window,sink", [(0, 0), (500, 4)])
+def test_chunk_many_blocks_per_cta(ops, window, sink):
+    """More blocks than CTAs, some of them with rows in the first of their two tiles only (and few tiles of the cache),
+    so that a CTA goes through many pieces."""
+    H, kvH = 40, 8
+    new = [33, 400, 21, 1, 230, 5, 50, 60] * 4
+    start = [(b * 379) % 1100 for b in range(len(new))]
+    c = R.Cache(ops, FP16, len(new), H, kvH, 1600, "paged", 128)
+    c.fill([s + n for s, n in zip(start, new)])
+    q = _randn((sum(new), H, D), FP16, 3)
+    out = _chunk(ops, c, q, new, start, window, sink)
+    _check_chunk(c, q, out, new, start, window, sink)
+    assert torch.equal(out, _chunk(ops, c, q, new, start, window, sink))
+
+
 def test_chunk_unseen_pages_need_not_exist(ops):
     new, start, window, sink = [140, 5], [800, 300], 150, 4
     c = R.Cache(ops, BF16, 2, 4, 2, 1024, "paged", 64)
