@@ -53,7 +53,9 @@ constexpr uint32_t kSmemExp = kSmemRaw + 2 * kRawBytes; // K [128], V [128]
 constexpr uint32_t kSmemRef = kSmemExp + 256;        // [4][r_k, r_v]
 constexpr uint32_t kSmemScan = kSmemRef + 32;        // 16 + 8 ints
 constexpr uint32_t kSmemBar = kSmemScan + 96;
-constexpr uint32_t kSmemTotal = kSmemBar + 256;
+constexpr uint32_t kSmemWalk = kSmemBar + 256;       // [16 warps]
+constexpr uint32_t kWalkBytes = 128;
+constexpr uint32_t kSmemTotal = kSmemWalk + 16 * kWalkBytes;
 static_assert(kSmemTotal <= 232448, "shared memory of one CTA");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256;
@@ -62,7 +64,7 @@ constexpr int kMaxCtas = 148;
 constexpr int kMaxBatch = 16000;                     // prefix sums of the batch lie in the Q tiles while a CTA finds its share
 
 enum { BAR_RAWFULL = 0, BAR_RAWEMPTY = 2, BAR_KFULL = 4, BAR_KEMPTY = 6, BAR_VFULL = 8, BAR_VEMPTY = 10, BAR_QFULL = 12, BAR_SFULL = 14,
-       BAR_PHALF = 16, BAR_PREADY = 18, BAR_ODONE = 20, BAR_REF = 22, BAR_QTAKEN = 26, BAR_COUNT = 28 };
+       BAR_PHALF = 16 /* [half][x] */, BAR_ODONE = 20, BAR_REF = 22, BAR_QTAKEN = 26, BAR_COUNT = 28 };
 static_assert(BAR_COUNT * 8 + 8 <= 256, "barrier block");
 
 using Block = Span<kBN>;
@@ -108,18 +110,47 @@ __device__ __forceinline__ int blocks_of(const Q8ChunkParams &cp, int b) {
   return (nq + 2 * cp.tile_tokens - 1) / (2 * cp.tile_tokens);
 }
 
+// The rows of tile X of a block: their positions, and which tiles of the walk they see.
+struct Half {
+  int first, n_tok;          // position of the first row; number of tokens (0: the tile is empty)
+  int fx, ex;                // besides the tiles of the first positions, tiles [fx, ex) of the walk hold something some row sees
+  int ga, gb;                // tiles [ga, gb), and the first `gs` ones: every row sees all of them
+  int gs;
+  __device__ __forceinline__ void of(const Q8ChunkParams &cp, const Block &s, int x) {
+    n_tok = max(0, min(cp.tile_tokens, s.nq - x * cp.tile_tokens));
+    first = s.pos0 + x * cp.tile_tokens;
+    const int last = min(first + n_tok, s.end) - 1;
+    const int skip = s.w0 - s.ns_tiles;  // walk index i >= ns_tiles is cache tile i + skip
+    fx = max(s.ns_tiles, window_begin(first, cp.a.window) / kBN - skip);
+    ex = n_tok > 0 ? min(s.n_tiles, last / kBN + 1 - skip) : 0;
+    ga = max(s.ns_tiles, (window_begin(first + n_tok - 1, cp.a.window) + kBN - 1) / kBN - skip);
+    gb = min(s.n_tiles, min(first + 1, s.end) / kBN - skip);
+    gs = min(s.ns_tiles, min(cp.a.n_sink, min(first + 1, s.end)) / kBN);
+    if (n_tok == 0 || last < 0) ex = 0, gs = gb = 0;
+  }
+  __device__ __forceinline__ bool sees(int i, int ns_tiles) const { return ex > 0 && (i < ns_tiles || (i >= fx && i < ex)); }
+  __device__ __forceinline__ bool sees_all(int i) const { return i < gs || (i >= ga && i < gb); }
+};
+
+// A warp's place in its CTA's share.  It lives in shared memory, one per warp: the registers belong to the
+// products and weights.  One lane moves it.
 struct Walk {
-  int b, blk, n_blk, kvh, i0, i1;
-  long left;
+  int b, blk, n_blk, kvh, i0, i1, left;
   Block s;
-  __device__ __forceinline__ void begin(const Q8ChunkParams &cp, int b_, int blk_, long offset, long tiles) {
+  Half hx[2];
+  __device__ __forceinline__ void block(const Q8ChunkParams &cp) {
+    s = block_of(cp, b, blk);
+    hx[0].of(cp, s, 0);
+    hx[1].of(cp, s, 1);
+  }
+  __device__ __forceinline__ void begin(const Q8ChunkParams &cp, int b_, int blk_, int offset, int tiles) {
     b = b_, blk = blk_;
     n_blk = blocks_of(cp, b);
-    s = block_of(cp, b, blk);
-    kvh = static_cast<int>(offset / s.n_tiles);
-    i0 = static_cast<int>(offset - static_cast<long>(kvh) * s.n_tiles);
+    block(cp);
+    kvh = offset / s.n_tiles;
+    i0 = offset - kvh * s.n_tiles;
     left = tiles;
-    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), i0 + left));
+    i1 = min(s.n_tiles, i0 + left);
   }
   __device__ __forceinline__ bool next(const Q8ChunkParams &cp) {
     left -= i1 - i0;
@@ -134,33 +165,21 @@ struct Walk {
             n_blk = blocks_of(cp, b);
           } while (n_blk == 0);
         }
-        s = block_of(cp, b, blk);
+        block(cp);
       } while (s.n_tiles == 0);
     }
     i0 = 0;
-    i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), left));
+    i1 = min(s.n_tiles, left);
     return true;
   }
 };
-
-// The rows of tile X of a block: their first and last positions, and which cache tiles they see.
-struct Half {
-  int first, last, n_tok;    // positions; number of tokens (0: the tile is empty)
-  int lo_first, lo_last;     // first window positions of the first and of the last row
-  __device__ __forceinline__ void of(const Q8ChunkParams &cp, const Block &s, int x) {
-    n_tok = max(0, min(cp.tile_tokens, s.nq - x * cp.tile_tokens));
-    first = s.pos0 + x * cp.tile_tokens;
-    last = first + n_tok - 1;
-    lo_first = window_begin(first, cp.a.window);
-    lo_last = window_begin(last, cp.a.window);
-  }
-  __device__ __forceinline__ bool sees(const Q8ChunkParams &cp, int col0) const { // some row, something of the tile
-    return n_tok > 0 && col0 <= last && (col0 + kBN > lo_first || col0 < cp.a.n_sink);
-  }
-  __device__ __forceinline__ bool sees_all(const Q8ChunkParams &cp, const Block &s, int col0) const { // every row, all of it
-    return col0 + kBN <= min(first + 1, s.end) && (col0 >= lo_last || col0 + kBN <= cp.a.n_sink);
-  }
-};
+__device__ __forceinline__ bool next_piece(Walk &w, const Q8ChunkParams &cp, int lane) { // all lanes
+  __syncwarp();
+  int more = 0;
+  if (lane == 0) more = w.next(cp);
+  __syncwarp();
+  return __shfl_sync(0xffffffffu, more, 0) != 0;
+}
 
 __device__ __forceinline__ int block_scan(int mine, int *scratch, int warp, int lane, int &total) { // exclusive; all threads
   int incl = mine;
@@ -181,6 +200,8 @@ __device__ __forceinline__ int block_scan(int mine, int *scratch, int warp, int 
   __syncthreads();
   return before;
 }
+
+static_assert(sizeof(Walk) <= kWalkBytes, "a warp's walk");
 
 } // namespace q8c
 
@@ -214,7 +235,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       mbar_init(bar(BAR_QFULL + s), 128);
       mbar_init(bar(BAR_SFULL + s), 1);
       mbar_init(bar(BAR_PHALF + s), 128);
-      mbar_init(bar(BAR_PREADY + s), 128);
+      mbar_init(bar(BAR_PHALF + 2 + s), 128);
       mbar_init(bar(BAR_ODONE + s), 1);
       mbar_init(bar(BAR_QTAKEN + s), 1);
     }
@@ -278,20 +299,19 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         scan[17] = u - prefix[b];
         scan[18] = static_cast<int>(x0 - at);
       }
-      if (u % gridDim.x == c) { // the CTAs share the writing of the merge's records
-        for (int h = 0; h < kvH; ++h) {
-          RunInfo r{};
-          r.c1 = -1;
-          if (s.n_tiles > 0) {
-            const long first = at + static_cast<long>(h) * s.n_tiles;
-            r.c0 = share_of(W, n, first);
-            r.c1 = share_of(W, n, first + s.n_tiles - 1);
-            r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) == first ? 0 : 1);
-          }
-          r.t0 = s.t0;
-          r.nq = s.nq;
-          cp.info[static_cast<long>(u) * kvH + h] = r;
+      for (int h = 0; h < kvH; ++h) { // the CTAs share the writing of the merge's records
+        if ((static_cast<unsigned>(u) * kvH + h) % gridDim.x != c) continue;
+        RunInfo r{};
+        r.c1 = -1;
+        if (s.n_tiles > 0) {
+          const long first = at + static_cast<long>(h) * s.n_tiles;
+          r.c0 = share_of(W, n, first);
+          r.c1 = share_of(W, n, first + s.n_tiles - 1);
+          r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) == first ? 0 : 1);
         }
+        r.t0 = s.t0;
+        r.nq = s.nq;
+        cp.info[static_cast<long>(u) * kvH + h] = r;
       }
       at += run;
     }
@@ -299,23 +319,23 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   if ((smem_base & 1023u) != 0 && tid == 0) report(err, 30);
   __syncthreads();
   if (c >= n || (smem_base & 1023u) != 0) return;
-  const int b_first = scan[16], blk_first = scan[17], off_first = scan[18];
+  const int b_first = scan[16], blk_first = scan[17], off_first = scan[18], share = static_cast<int>(x1 - x0);
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t *>(tmem_slot))), "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  Walk &w = *reinterpret_cast<Walk *>(smem + kSmemWalk + warp * kWalkBytes);
+  if (lane == 0) w.begin(cp, b_first, blk_first, off_first, share);
   tc_fence_before();
   __syncthreads(); // also: the prefix sums in the Q tiles are done with
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
-    reg_dec<64>();
-    Walk w;
+    reg_dec<96>();
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
-      w.begin(cp, b_first, blk_first, off_first, x1 - x0);
       uint32_t g = 0;
       bool ok = true;
       do {
@@ -374,19 +394,19 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
           }
         }
-      } while (ok && w.next(cp));
+      } while (ok && next_piece(w, cp, lane));
     } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------- MMA issuer
-      w.begin(cp, b_first, blk_first, off_first, x1 - x0);
       constexpr uint32_t idesc_qk = instr_desc(0u, 0), idesc_pv = instr_desc(0u, 1);
       const uint32_t dq0 = smem_desc_lo(smem_base + kSmemQ, 16);
       const uint32_t dk0 = smem_desc_lo(smem_base + kSmemK, 16);
       const uint32_t dv0 = smem_desc_lo(smem_base + kSmemV, kHalfTile);
       constexpr uint32_t kTileStep = kTileBytes >> 4, kHalfStep = kHalfTile >> 4;
       uint32_t g = 0;                 // tiles of the share so far
-      uint32_t cnt[2] = {0, 0};       // P.V products issued for A and B
       int piece = 0;
       bool ok = true;
+      // The loops over A and B are not unrolled: the instructions of all roles have to fit the
+      // instruction cache together.
       auto issue_qk = [&](int x, uint32_t gt) {
         const uint32_t d = tmem + kColS + 128 * x, dq = dq0 + x * kTileStep, dk = dk0 + (gt & 1) * kTileStep;
 #pragma unroll
@@ -396,118 +416,118 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         }
         tc_commit(bar(BAR_SFULL + x));
       };
-      auto issue_pv = [&](int x, uint32_t gt, bool first) -> bool {
-        if (!mbar_wait(bar(BAR_PHALF + x), cnt[x] & 1, abort_flag, err, 10)) return false;
-        if (!mbar_wait(bar(BAR_VFULL + (gt & 1)), (gt >> 1) & 1, abort_flag, err, 6)) return false;
-        tc_fence_after();
+      auto issue_pv = [&](int x, uint32_t gt, uint32_t ph, uint32_t acc) -> bool {
         const uint32_t pcol = tmem + kColS + 128 * x, ocol = tmem + kColO + 128 * x;
         const uint32_t dv = dv0 + (gt & 1) * kTileStep;
-        const uint32_t acc0 = first ? 0u : 1u;
+        if (!mbar_wait(bar(BAR_VFULL + (gt & 1)), (gt >> 1) & 1, abort_flag, err, 6)) return false;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) { // the first 64 positions of P are published before the others
+          if (!mbar_wait(bar(BAR_PHALF + 2 * h + x), ph, abort_flag, err, 10)) return false;
+          tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_ts(ocol, pcol + 8 * k, dv + k * (2048 >> 4), kDescHi, idesc_pv, k > 0 ? 1u : acc0);
-        if (!mbar_wait(bar(BAR_PREADY + x), cnt[x] & 1, abort_flag, err, 5)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 4; k < 8; ++k) tc_mma_ts(ocol, pcol + 8 * k, dv + k * (2048 >> 4), kDescHi, idesc_pv, 1u);
+          for (int k = 0; k < 4; ++k) {
+            tc_mma_ts(ocol, pcol + 32 * h + 8 * k, dv + (4 * h + k) * (2048 >> 4), kDescHi, idesc_pv, acc);
+            acc = 1u;
+          }
+        }
         tc_commit(bar(BAR_ODONE + x));
-        ++cnt[x];
         return true;
       };
+      uint32_t cnt = 0;               // bit x: parity of the P.V products issued for tile x
       do {
-        Half hx[2];
-        hx[0].of(cp, w.s, 0);
-        hx[1].of(cp, w.s, 1);
-        bool begun[2] = {false, false};
-        // K of the piece's first tile, and the rows of Q (their writers have also taken the previous results out)
-        ok = mbar_wait(bar(BAR_KFULL + (g & 1)), (g >> 1) & 1, abort_flag, err, 4);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          ok = ok && mbar_wait(bar(BAR_QFULL + x), piece & 1, abort_flag, err, 3);
-          if (!ok) break;
-          mbar_arrive(bar(BAR_QTAKEN + x));
-          tc_fence_after();
-          if (hx[x].sees(cp, w.s.tile(w.i0) * kBN)) issue_qk(x, g);
-        }
-        if (ok) tc_commit(bar(BAR_KEMPTY + (g & 1)));
-        for (int i = w.i0; ok && i < w.i1; ++i, ++g) {
-          const int col0 = w.s.tile(i) * kBN;
-          const bool more = i + 1 < w.i1;
-          const int col1 = more ? w.s.tile(i + 1) * kBN : 0;
-          if (more) ok = mbar_wait(bar(BAR_KFULL + ((g + 1) & 1)), ((g + 1) >> 1) & 1, abort_flag, err, 4);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (ok && hx[x].sees(cp, col0)) {
-              ok = issue_pv(x, g, !begun[x]);
-              begun[x] = true;
+        const int i0 = w.i0, i1 = w.i1, ns_tiles = w.s.ns_tiles;
+        const int fa = w.hx[0].fx, ea = w.hx[0].ex, fb = w.hx[1].fx, eb = w.hx[1].ex;
+        auto sees = [&](int x, int i) { const int e = x ? eb : ea; return e > 0 && (i < ns_tiles || (i >= (x ? fb : fa) && i < e)); };
+        uint32_t begun = 0;
+        // step i: P.V of tile i, then Q.K of tile i + 1, for A and for B
+        for (int i = i0 - 1; ok && i < i1; ++i) {
+          const bool more = i + 1 < i1;
+          const uint32_t gk = g + static_cast<uint32_t>(i + 1 - i0), gv = gk - 1;
+          if (more) ok = mbar_wait(bar(BAR_KFULL + (gk & 1)), (gk >> 1) & 1, abort_flag, err, 4);
+#pragma unroll 1
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (i < i0) { // the rows of Q; their writers have also taken the previous piece's results out
+              ok = mbar_wait(bar(BAR_QFULL + x), piece & 1, abort_flag, err, 3);
+              mbar_arrive(bar(BAR_QTAKEN + x));
+            } else if (sees(x, i)) {
+              ok = issue_pv(x, gv, (cnt >> x) & 1, (begun >> x) & 1);
+              cnt ^= 1u << x;
+              begun |= 1u << x;
             }
-            if (ok && more && hx[x].sees(cp, col1)) {
+            if (ok && more && sees(x, i + 1)) {
               tc_fence_after();
-              issue_qk(x, g + 1);
+              issue_qk(x, gk);
             }
           }
-          if (ok) {
-            ok = mbar_wait(bar(BAR_VFULL + (g & 1)), (g >> 1) & 1, abort_flag, err, 6); // a stage is freed only after it was filled
-            tc_commit(bar(BAR_VEMPTY + (g & 1)));
-            if (more) tc_commit(bar(BAR_KEMPTY + ((g + 1) & 1)));
+          if (!ok) break;
+          if (i >= i0) {
+            ok = mbar_wait(bar(BAR_VFULL + (gv & 1)), (gv >> 1) & 1, abort_flag, err, 6); // a stage is freed only after it was filled
+            tc_commit(bar(BAR_VEMPTY + (gv & 1)));
           }
+          if (more) tc_commit(bar(BAR_KEMPTY + (gk & 1)));
         }
+        g += static_cast<uint32_t>(i1 - i0);
         ++piece;
       } while (ok && w.next(cp));
     }
   } else if (warp < 12) {
-    reg_inc<184>();
+    reg_inc<160>();
     // ------------------------------------------------------------ softmax, Q and results of tile X
     const int x = (warp >> 2) - 1, quad = warp & 3;
     const int r = quad * 32 + lane;              // row of the tile
     const int tok = r / G, hd = r - tok * G;     // its token and head of the group
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t scol = tmem + lane_addr + kColS + 128 * x, ocol = tmem + lane_addr + kColO + 128 * x;
-    Walk w;
-    w.begin(cp, b_first, blk_first, off_first, x1 - x0);
     uint32_t g = 0, cnt = 0;
     int piece = 0;
     bool ok = true;
     do {
-      Half hx;
-      hx.of(cp, w.s, x);
+      const Half &hx = w.hx[x];
       const bool live = tok < hx.n_tok;          // tok < tile_tokens for every row that exists
       const long t = static_cast<long>(w.s.t0) + x * cp.tile_tokens + tok;
       // a tile that sees nothing of a piece must not run more than one piece ahead of the MMA warp
       if (piece > 0 && !__all_sync(0xffffffffu, mbar_wait(bar(BAR_QTAKEN + x), (piece - 1) & 1, abort_flag, err, 13))) break;
       // ---- the row of Q, scaled to fp16: its largest magnitude to 2^13 .. 2^14
-      float rowc;
+      float rowc, up;
       {
-        uint4 u[16];
-        uint32_t top = 0;
         const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + t * p.q_row + (w.kvh * G + hd) * kHeadDim);
+        uint32_t top = 0;
+#pragma unroll 1
+        for (int i = 0; i < 16; i += 8) {
+          uint4 u[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) u[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < 8; ++k) u[k] = live ? src[i + k] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t *wd = reinterpret_cast<const uint32_t *>(&u[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = Elem<T>::unpack(wd[e]);
-            top = max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+          for (int k = 0; k < 8; ++k) {
+            // magnitudes of 16-bit floats order like their bit patterns
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(u[k].x & 0x7fff7fffu, u[k].y & 0x7fff7fffu), __vmaxu2(u[k].z & 0x7fff7fffu, u[k].w & 0x7fff7fffu)));
           }
         }
-        int e = max(static_cast<int>(top >> 23) - 127, -100);
-        if (top >= 0x7f800000u) e = 13;          // not finite: as it is
-        const float up = pow2i(13 - e);
+        const float2 two = Elem<T>::unpack(max(top & 0xffffu, top >> 16));
+        const uint32_t topf = __float_as_uint(two.x) & 0x7fffffffu;
+        int e = max(static_cast<int>(topf >> 23) - 127, -100);
+        if (topf >= 0x7f800000u) e = 13;         // not finite: as it is
+        up = pow2i(13 - e);
         rowc = p.scale_log2 * pow2i(e - 13);
         const uint32_t dst = smem_base + kSmemQ + x * kTileBytes + r * 128;
+#pragma unroll 1
+        for (int i = 0; i < 16; i += 4) {
+          uint4 u[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          uint32_t *wd = reinterpret_cast<uint32_t *>(&u[i]);
+          for (int k = 0; k < 4; ++k) u[k] = live ? src[i + k] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            const float2 v = Elem<T>::unpack(wd[e2]);
-            wd[e2] = Elem<__half>::pack(v.x * up, v.y * up);
+          for (int k = 0; k < 4; ++k) {
+            uint32_t *wd = reinterpret_cast<uint32_t *>(&u[k]);
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) {
+              const float2 v = Elem<T>::unpack(wd[e2]);
+              wd[e2] = Elem<__half>::pack(v.x * up, v.y * up);
+            }
+            const uint32_t chunk = static_cast<uint32_t>((i + k) & 7) ^ static_cast<uint32_t>(r & 7);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kHalfTile + (chunk << 4)), "r"(u[k].x), "r"(u[k].y),
+                         "r"(u[k].z), "r"(u[k].w)
+                         : "memory");
           }
-          const uint32_t chunk = static_cast<uint32_t>(i & 7) ^ static_cast<uint32_t>(r & 7);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kHalfTile + (chunk << 4)), "r"(u[i].x), "r"(u[i].y),
-                       "r"(u[i].z), "r"(u[i].w)
-                       : "memory");
         }
       }
       fence_proxy_async_smem();
@@ -516,11 +536,11 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 
       const int pos = hx.first + tok;
       const int vend = live ? min(pos + 1, w.s.end) : 0, wlo = window_begin(pos, p.window);
+      const int i0 = w.i0, i1 = w.i1, ns_tiles = w.s.ns_tiles;
       float m_ref = -INFINITY, l = 0.f;
       bool begun = false;
-      for (int i = w.i0; i < w.i1; ++i, ++g) {
-        const int col0 = w.s.tile(i) * kBN;
-        if (!hx.sees(cp, col0)) continue;
+      for (int i = i0; i < i1; ++i, ++g) {
+        if (!hx.sees(i, ns_tiles)) continue;
         ok = ok && mbar_wait(bar(BAR_SFULL + x), cnt & 1, abort_flag, err, 7);
         ok = ok && mbar_wait(bar(BAR_REF + (g & 3)), (g >> 2) & 1, abort_flag, err, 12); // complete by now: K was converted before S
         if (!__all_sync(0xffffffffu, ok)) {
@@ -530,26 +550,37 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         tc_fence_after();
         const int rk = refs[2 * (g & 3)], rv = refs[2 * (g & 3) + 1];
         const float a = fmaxf(rowc * pow2i(rk - 7), 1.2e-38f), off = static_cast<float>(rv - 7);
-        uint32_t su[128];
+        const bool all = hx.sees_all(i);
+        const int col0 = w.s.tile(i) * kBN;
+        // hides what the row does not see of 64 columns from column 64 h
+        auto hide = [&](uint32_t (&v)[64], int h) {
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) tc_ld32(scol + 32 * q4, su + 32 * q4);
-        tc_wait_ld();
-        if (!hx.sees_all(cp, w.s, col0)) {
-          const int ve = vend - col0, wl = wlo - col0, sk = p.n_sink - col0;
+          for (int q = 0; q < 2; ++q) {
+            const int c0 = col0 + 64 * h + 32 * q;
+            auto below = [&](int k) { return k - c0 <= 0 ? 0u : k - c0 >= 32 ? 0xffffffffu : (1u << (k - c0)) - 1u; }; // columns < k
+            const uint32_t vis = below(vend) & (~below(wlo) | below(p.n_sink));
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (!(j < ve && (j >= wl || j < sk))) su[j] = 0xff800000u; // -inf
+            for (int j = 0; j < 32; ++j)
+              if (!(vis & (1u << j))) v[32 * q + j] = 0xff800000u; // -inf
+          }
+        };
+        // The row is read twice, for its maximum and for its weights, 64 columns at a time: kept whole it
+        // would not fit the registers, and unrolled whole the instructions would not fit their cache.
+        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t su[64];
+          tc_ld32(scol + 64 * h, su);
+          tc_ld32(scol + 64 * h + 32, su + 32);
+          tc_wait_ld();
+          if (!all) hide(su, h);
+#pragma unroll
+          for (int j = 0; j < 64; j += 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mxa[k] = max3(mxa[k], __uint_as_float(su[j + k]), __uint_as_float(su[j + 4 + k]));
+          }
         }
-        float mxa[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mxa[j] = fmaxf(__uint_as_float(su[j]), __uint_as_float(su[8 + j]));
-#pragma unroll
-        for (int j = 16; j < 128; j += 16) {
-#pragma unroll
-          for (int q8i = 0; q8i < 8; ++q8i) mxa[q8i] = max3(mxa[q8i], __uint_as_float(su[j + q8i]), __uint_as_float(su[j + 8 + q8i]));
-        }
-        const float top = fmaxf(max3(mxa[0], mxa[1], mxa[2]), fmaxf(max3(mxa[3], mxa[4], mxa[5]), fmaxf(mxa[6], mxa[7])));
-        const float mx = fmaf(top, a, off);
+        const float mx = fmaf(fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])), a, off);
         const bool grow = mx > m_ref + kLazy;
         if (__any_sync(0xffffffffu, grow) && begun) {
           if (!__all_sync(0xffffffffu, mbar_wait(bar(BAR_ODONE + x), (cnt - 1) & 1, abort_flag, err, 8))) {
@@ -559,7 +590,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           tc_fence_after();
           const float f = grow ? ex2(m_ref - mx) : 1.f;
           l *= f;
-#pragma unroll
+#pragma unroll 1
           for (int q4 = 0; q4 < 4; ++q4) {
             uint32_t o[32];
             tc_ld32(ocol + 32 * q4, o);
@@ -573,23 +604,28 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         if (grow) m_ref = mx;
         begun = true;
         const float nm = off - (m_ref == -INFINITY ? 0.f : m_ref); // nothing seen yet: P = 0
-        uint32_t pk[64];
         uint64_t sums[2] = {0ull, 0ull};
         const uint64_t a2 = pack2(a, a), nm2 = pack2(nm, nm);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t su[64], pk[32];
+          tc_ld32(scol + 64 * h, su);
+          tc_ld32(scol + 64 * h + 32, su + 32);
+          tc_wait_ld();
+          if (!all) hide(su, h);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          const uint64_t y2 = fma2(pack2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), a2, nm2);
-          float y0, y1;
-          unpack2(y2, y0, y1);
-          const float e0 = ex2(y0), e1 = ex2(y1);
-          sums[j & 1] = add2(sums[j & 1], pack2(e0, e1));
-          pk[j] = Elem<__half>::pack(e0, e1);
-          if (j == 31) {
-            tc_st32(scol, pk);
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(bar(BAR_PHALF + x));
+          for (int j = 0; j < 32; ++j) {
+            const uint64_t y2 = fma2(pack2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), a2, nm2);
+            float y0, y1;
+            unpack2(y2, y0, y1);
+            const float e0 = ex2(y0), e1 = ex2(y1);
+            sums[j & 1] = add2(sums[j & 1], pack2(e0, e1));
+            pk[j] = Elem<__half>::pack(e0, e1);
           }
+          tc_st32(scol + 32 * h, pk); // 64 fp16 weights over columns of S that have been read
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(BAR_PHALF + 2 * h + x));
         }
         {
           float s0, s1, s2, s3;
@@ -597,10 +633,6 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           unpack2(sums[1], s2, s3);
           l = fmaf((s0 + s1) + (s2 + s3), pow2i(7 - rv), l);
         }
-        tc_st32(scol + 32, pk + 32);
-        tc_wait_st();
-        tc_fence_before();
-        mbar_arrive(bar(BAR_PREADY + x));
         ++cnt;
       }
       if (!ok) break;
@@ -614,7 +646,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       const float inv = l == 0.f ? 0.f : 1.f / l;  // NaN stays NaN
       const long slot_row = static_cast<long>(2 * c + (piece == 0 ? 0 : 1)) * (tok2 * G) + (x * cp.tile_tokens + tok) * G + hd;
       T *dst = static_cast<T *>(p.out) + t * p.out_row + (w.kvh * G + hd) * kHeadDim;
-#pragma unroll
+#pragma unroll 1
       for (int q4 = 0; q4 < 4; ++q4) {
         uint32_t o[32];
         if (begun) {
@@ -645,38 +677,46 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       }
       if (live && !whole) cp.lse[slot_row] = l == 0.f ? -INFINITY : (m_ref == -INFINITY ? 0.f : m_ref) + log2f(l);
       ++piece;
-    } while (w.next(cp));
+    } while (next_piece(w, cp, lane));
   } else {
-    reg_dec<80>();
+    reg_dec<96>();
     // ------------------------------------------------------------ converters: 32 rows of every tile per warp
     const int cw = warp - 12;
-    Walk w;
-    w.begin(cp, b_first, blk_first, off_first, x1 - x0);
     uint32_t g = 0;
     bool ok = true;
     // rows 32 cw .. 32 cw + 31 of the raw tile -> fp16 operand tile; `f`: this lane's row's factor, two fp16 (0: zeros)
     auto convert = [&](uint32_t raw, uint32_t dst, uint32_t f) {
-#pragma unroll 4
-      for (int it = 0; it < 8; ++it) {
-        const int rl = it * 4 + (lane >> 3), row = 32 * cw + rl, ch = lane & 7; // 16 codes: elements 16 ch ..
-        const uint32_t fr = __shfl_sync(0xffffffffu, f, rl);
-        uint32_t wv[4], h[8];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(wv[0]), "=r"(wv[1]), "=r"(wv[2]), "=r"(wv[3]) : "r"(raw + row * 128 + ch * 16));
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        uint32_t wv[4][4]; // sixteen rows are under way at once
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t v = hmul2(cvt_e4m3x2_f16x2((wv[e >> 1] >> (16 * (e & 1))) & 0xffffu), fr);
-          h[e] = fr ? v : 0u;
+        for (int it = 0; it < 4; ++it) {
+          const int row = 32 * cw + half * 16 + it * 4 + (lane >> 3);
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(wv[it][0]), "=r"(wv[it][1]), "=r"(wv[it][2]), "=r"(wv[it][3])
+                       : "r"(raw + row * 128 + (lane & 7) * 16));
         }
-        // two 16-byte chunks of the row's half tile; lanes of the two halves write them in opposite order
-        // (the halves lie 16 KB apart, in the same banks)
-        const uint32_t base = dst + (ch >> 2) * kHalfTile + row * 128, c0 = 2 * (ch & 3), flip = ch >> 2;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t q = k ^ flip;
-          const uint32_t at = base + (((c0 + q) ^ (row & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q ? h[4] : h[0]), "r"(q ? h[5] : h[1]), "r"(q ? h[6] : h[2]),
-                       "r"(q ? h[7] : h[3])
-                       : "memory");
+        for (int it = 0; it < 4; ++it) {
+          const int rl = half * 16 + it * 4 + (lane >> 3), row = 32 * cw + rl, ch = lane & 7; // elements 16 ch ..
+          const uint32_t fr = __shfl_sync(0xffffffffu, f, rl);
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t v = hmul2(cvt_e4m3x2_f16x2((wv[it][e >> 1] >> (16 * (e & 1))) & 0xffffu), fr);
+            h[e] = fr ? v : 0u;
+          }
+          // two 16-byte chunks of the row's half tile; lanes of the two halves write them in opposite order
+          // (the halves lie 16 KB apart, in the same banks)
+          const uint32_t base = dst + (ch >> 2) * kHalfTile + row * 128, c0 = 2 * (ch & 3), flip = ch >> 2;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t q = k ^ flip;
+            const uint32_t at = base + (((c0 + q) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q ? h[4] : h[0]), "r"(q ? h[5] : h[1]), "r"(q ? h[6] : h[2]),
+                         "r"(q ? h[7] : h[3])
+                         : "memory");
+          }
         }
       }
     };
@@ -708,31 +748,29 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const bool vis = seen(col0 + row), poison = kx == kPoison || vx == kPoison;
         const uint32_t fk = !vis ? 0u : poison ? 0x7e007e00u : factor(rk - kx);
         const uint32_t fv = !vis || poison ? 0u : factor(rv - vx);
-        ok = mbar_wait(bar(BAR_KEMPTY + s), sph ^ 1, abort_flag, err, 21);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        convert(smem_base + kSmemRaw, smem_base + kSmemK + s * kTileBytes, fk);
-        if (cw == 0 && lane == 0) {
-          refs[2 * (g & 3)] = rk - 127;
-          refs[2 * (g & 3) + 1] = rv - 127;
-          mbar_arrive(bar(BAR_REF + (g & 3)));
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(BAR_KFULL + s));
-          mbar_arrive(bar(BAR_RAWEMPTY + 0));
-        }
-        ok = mbar_wait(bar(BAR_RAWFULL + 1), ph, abort_flag, err, 22) && mbar_wait(bar(BAR_VEMPTY + s), sph ^ 1, abort_flag, err, 23);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        convert(smem_base + kSmemRaw + kRawBytes, smem_base + kSmemV + s * kTileBytes, fv);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(BAR_VFULL + s));
-          mbar_arrive(bar(BAR_RAWEMPTY + 1));
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          if (kv) ok = mbar_wait(bar(BAR_RAWFULL + 1), ph, abort_flag, err, 22);
+          ok = ok && mbar_wait(bar((kv ? BAR_VEMPTY : BAR_KEMPTY) + s), sph ^ 1, abort_flag, err, 21);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          convert(smem_base + kSmemRaw + kv * kRawBytes, smem_base + (kv ? kSmemV : kSmemK) + s * kTileBytes, kv ? fv : fk);
+          if (kv == 0 && cw == 0 && lane == 0) {
+            refs[2 * (g & 3)] = rk - 127;
+            refs[2 * (g & 3) + 1] = rv - 127;
+            mbar_arrive(bar(BAR_REF + (g & 3)));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar((kv ? BAR_VFULL : BAR_KFULL) + s));
+            mbar_arrive(bar(BAR_RAWEMPTY + kv));
+          }
         }
       }
-    } while (__all_sync(0xffffffffu, ok) && w.next(cp));
+    } while (__all_sync(0xffffffffu, ok) && next_piece(w, cp, lane));
   }
   tc_fence_before();
   __syncthreads();
