@@ -10,7 +10,7 @@
 //
 // 16 warps in four groups:
 //   warp 0       TMA producer: e4m3 tiles of K and V in boxes of 64 positions, with their exponents
-//   warp 1       MMA issuer: S_X = Q_X K^T, then O_X += P_X V with P from tensor memory
+//   warps 1, 2   MMA issuers of A and B: S_X = Q_X K^T, then O_X += P_X V with P from tensor memory
 //   warps 4-11   softmax of tile A (4-7) and B (8-11), one thread per query row; they also bring the
 //                rows of Q in and the results out
 //   warps 12-15  converters: e4m3 -> fp16 operand tiles
@@ -53,19 +53,21 @@ constexpr uint32_t kSmemExp = kSmemRaw + 2 * kRawBytes; // K [128], V [128]
 constexpr uint32_t kSmemRef = kSmemExp + 256;        // [4][r_k, r_v]
 constexpr uint32_t kSmemScan = kSmemRef + 32;        // 16 + 8 ints
 constexpr uint32_t kSmemBar = kSmemScan + 96;
-constexpr uint32_t kSmemWalk = kSmemBar + 256;       // [16 warps]
+constexpr uint32_t kSmemWalk = kSmemBar + 320;       // [16 warps]
 constexpr uint32_t kWalkBytes = 128;
 constexpr uint32_t kSmemTotal = kSmemWalk + 16 * kWalkBytes;
 static_assert(kSmemTotal <= 232448, "shared memory of one CTA");
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 0, kColO = 256;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256; // S_X: 64 columns at kColS + 64 X; P_X: two halves of 32 at kColP + 64 X; O_X
 constexpr float kLazy = 8.0f;
 constexpr int kMaxCtas = 148;
+constexpr int kPieceCost = 6;                        // what a block costs besides its tiles, in tiles: its rows of Q, fill and drain, results.
+                                                     // Prompts of 33 to 1024 tokens: 520 us with 0, 359 with 2, 312 with 4, 309 with 8
 constexpr int kMaxBatch = 16000;                     // prefix sums of the batch lie in the Q tiles while a CTA finds its share
 
-enum { BAR_RAWFULL = 0, BAR_RAWEMPTY = 2, BAR_KFULL = 4, BAR_KEMPTY = 6, BAR_VFULL = 8, BAR_VEMPTY = 10, BAR_QFULL = 12, BAR_SFULL = 14,
-       BAR_PHALF = 16 /* [half][x] */, BAR_ODONE = 20, BAR_REF = 22, BAR_QTAKEN = 26, BAR_COUNT = 28 };
-static_assert(BAR_COUNT * 8 + 8 <= 256, "barrier block");
+enum { BAR_RAWFULL = 0, BAR_RAWEMPTY = 2, BAR_KFULL = 4, BAR_KEMPTY = 6, BAR_VFULL = 8, BAR_VEMPTY = 10, BAR_QFULL = 12, BAR_QTAKEN = 14,
+       BAR_SFULL = 16, BAR_SFREE = 18, BAR_PFULL = 20 /* [half][x] */, BAR_ODONE = 24 /* [half][x] */, BAR_REF = 28, BAR_COUNT = 32 };
+static_assert(BAR_COUNT * 8 + 8 <= 320, "barrier block");
 
 using Block = Span<kBN>;
 
@@ -143,14 +145,17 @@ struct Walk {
     hx[0].of(cp, s, 0);
     hx[1].of(cp, s, 1);
   }
-  __device__ __forceinline__ void begin(const Q8ChunkParams &cp, int b_, int blk_, int offset, int tiles) {
+  // `offset`: the share's begin on the runs of this block's KV heads; a run is kPieceCost, then its tiles
+  __device__ __forceinline__ bool begin(const Q8ChunkParams &cp, int b_, int blk_, int offset, int share) {
     b = b_, blk = blk_;
     n_blk = blocks_of(cp, b);
     block(cp);
-    kvh = offset / s.n_tiles;
-    i0 = offset - kvh * s.n_tiles;
-    left = tiles;
+    kvh = offset / (s.n_tiles + kPieceCost);
+    const int at = offset - kvh * (s.n_tiles + kPieceCost);
+    i0 = max(0, at - kPieceCost);
+    left = share - max(0, kPieceCost - at);
     i1 = min(s.n_tiles, i0 + left);
+    return left > 0;
   }
   __device__ __forceinline__ bool next(const Q8ChunkParams &cp) {
     left -= i1 - i0;
@@ -168,9 +173,10 @@ struct Walk {
         block(cp);
       } while (s.n_tiles == 0);
     }
+    left -= kPieceCost;
     i0 = 0;
     i1 = min(s.n_tiles, left);
-    return true;
+    return left > 0;
   }
 };
 __device__ __forceinline__ bool next_piece(Walk &w, const Q8ChunkParams &cp, int lane) { // all lanes
@@ -179,6 +185,12 @@ __device__ __forceinline__ bool next_piece(Walk &w, const Q8ChunkParams &cp, int
   if (lane == 0) more = w.next(cp);
   __syncwarp();
   return __shfl_sync(0xffffffffu, more, 0) != 0;
+}
+
+// mbar_wait with the waiting itself out of the way of the instructions that follow
+__device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, int *error_flag, int code) {
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+  return mbar_wait(bar, parity, abort_flag, error_flag, code);
 }
 
 __device__ __forceinline__ int block_scan(int mine, int *scratch, int warp, int lane, int &total) { // exclusive; all threads
@@ -229,15 +241,17 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       mbar_init(bar(BAR_RAWFULL + s), 1);
       mbar_init(bar(BAR_RAWEMPTY + s), 4);
       mbar_init(bar(BAR_KFULL + s), 4);
-      mbar_init(bar(BAR_KEMPTY + s), 1);
+      mbar_init(bar(BAR_KEMPTY + s), 2);
       mbar_init(bar(BAR_VFULL + s), 4);
-      mbar_init(bar(BAR_VEMPTY + s), 1);
+      mbar_init(bar(BAR_VEMPTY + s), 2);
       mbar_init(bar(BAR_QFULL + s), 128);
-      mbar_init(bar(BAR_SFULL + s), 1);
-      mbar_init(bar(BAR_PHALF + s), 128);
-      mbar_init(bar(BAR_PHALF + 2 + s), 128);
-      mbar_init(bar(BAR_ODONE + s), 1);
       mbar_init(bar(BAR_QTAKEN + s), 1);
+      mbar_init(bar(BAR_SFULL + s), 1);
+      mbar_init(bar(BAR_SFREE + s), 128);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(bar(BAR_PFULL + 2 * h + s), 128);
+        mbar_init(bar(BAR_ODONE + 2 * h + s), 1);
+      }
     }
     for (int s = 0; s < 4; ++s) mbar_init(bar(BAR_REF + s), 1);
     *abort_flag = 0;
@@ -279,7 +293,8 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   int mine = 0;
   for (int u = u_lo, b = b_lo; u < u_hi; ++u) {
     while (u >= prefix[b + 1]) ++b;
-    mine += block_of(cp, b, u - prefix[b]).n_tiles;
+    const int tiles = block_of(cp, b, u - prefix[b]).n_tiles;
+    mine += tiles > 0 ? tiles + kPieceCost : 0;
   }
   int total;
   const int before = block_scan(mine, scan, warp, lane, total);
@@ -293,7 +308,8 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     for (int u = u_lo, b = b_lo; u < u_hi; ++u) {
       while (u >= prefix[b + 1]) ++b;
       const Block s = block_of(cp, b, u - prefix[b]);
-      const long run = static_cast<long>(s.n_tiles) * kvH;
+      const int one = s.n_tiles > 0 ? s.n_tiles + kPieceCost : 0;
+      const long run = static_cast<long>(one) * kvH;
       if (x0 >= at && x0 < at + run) {
         scan[16] = b;
         scan[17] = u - prefix[b];
@@ -304,10 +320,10 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         RunInfo r{};
         r.c1 = -1;
         if (s.n_tiles > 0) {
-          const long first = at + static_cast<long>(h) * s.n_tiles;
-          r.c0 = share_of(W, n, first);
-          r.c1 = share_of(W, n, first + s.n_tiles - 1);
-          r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) == first ? 0 : 1);
+          const long first = at + static_cast<long>(h) * one;
+          r.c0 = share_of(W, n, first + kPieceCost);
+          r.c1 = share_of(W, n, first + one - 1);
+          r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) >= first ? 0 : 1);
         }
         r.t0 = s.t0;
         r.nq = s.nq;
@@ -320,13 +336,15 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   __syncthreads();
   if (c >= n || (smem_base & 1023u) != 0) return;
   const int b_first = scan[16], blk_first = scan[17], off_first = scan[18], share = static_cast<int>(x1 - x0);
+  Walk &w = *reinterpret_cast<Walk *>(smem + kSmemWalk + warp * kWalkBytes);
+  int some = 0;
+  if (lane == 0) some = w.begin(cp, b_first, blk_first, off_first, share);
+  if (!__syncthreads_or(some)) return; // the share is all cost and no tile
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t *>(tmem_slot))), "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  Walk &w = *reinterpret_cast<Walk *>(smem + kSmemWalk + warp * kWalkBytes);
-  if (lane == 0) w.begin(cp, b_first, blk_first, off_first, share);
   tc_fence_before();
   __syncthreads(); // also: the prefix sums in the Q tiles are done with
   tc_fence_after();
@@ -368,7 +386,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             if (lane == 0) {
 #pragma unroll
               for (int kv = 0; kv < 2; ++kv) {
-                ok = ok && mbar_wait(bar(BAR_RAWEMPTY + kv), (g & 1) ^ 1, abort_flag, err, 1);
+                ok = ok && await(bar(BAR_RAWEMPTY + kv), (g & 1) ^ 1, abort_flag, err, 1);
                 if (!ok) break;
                 const uint32_t full = bar(BAR_RAWFULL + kv);
                 uint32_t bytes = 0, xb[2];
@@ -395,89 +413,111 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           }
         }
       } while (ok && next_piece(w, cp, lane));
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------- MMA issuer
-      constexpr uint32_t idesc_qk = instr_desc(0u, 0), idesc_pv = instr_desc(0u, 1);
-      const uint32_t dq0 = smem_desc_lo(smem_base + kSmemQ, 16);
-      const uint32_t dk0 = smem_desc_lo(smem_base + kSmemK, 16);
-      const uint32_t dv0 = smem_desc_lo(smem_base + kSmemV, kHalfTile);
-      constexpr uint32_t kTileStep = kTileBytes >> 4, kHalfStep = kHalfTile >> 4;
-      uint32_t g = 0;                 // tiles of the share so far
-      int piece = 0;
+    } else if (warp < 3) {
+      // ---------------------------------------------------------- MMA issuer of tile X
+      // One warp each for A and B.  A tile is taken in two steps of 64 positions.  The softmax warps
+      // copy a step's scores to registers and free them at once, so that the next step's scores are
+      // made while they work: Q.K of step n + 1 goes before P.V of step n.
+      // The whole warp walks through this, on values that are visibly the same in all lanes, and one
+      // elected lane issues: the descriptors then live in uniform registers, from where the products
+      // take them; a lone lane has to move six values there for each product.
+      const int x = __shfl_sync(0xffffffffu, warp, 0) - 1;
+      constexpr uint32_t idesc_qk = (instr_desc(0u, 0) & ~(0x3fu << 17)) | ((64u >> 3) << 17), idesc_pv = instr_desc(0u, 1);
+      constexpr uint32_t kTileStep = kTileBytes >> 4, kHalfStep = kHalfTile >> 4, kRows64 = (64 * 128) >> 4;
+      const uint32_t base_u = __shfl_sync(0xffffffffu, smem_base, 0), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t dq0 = smem_desc_lo(base_u + kSmemQ, 16) + x * kTileStep;
+      const uint32_t dk0 = smem_desc_lo(base_u + kSmemK, 16);
+      const uint32_t dv0 = smem_desc_lo(base_u + kSmemV, kHalfTile);
+      const uint32_t scol = tmem_u + kColS + 64 * x, pcol = tmem_u + kColP + 64 * x, ocol = tmem_u + kColO + 128 * x;
+      const uint32_t bars = base_u + kSmemBar;
+      auto ubar = [&](int i) { return bars + 8u * i; };
+      auto wait = [&](int i, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, await(ubar(i), parity, abort_flag, err, code));
+      };
+      const bool leader = elect_one();
+      uint32_t gk = 0, gv = 0;        // tiles of the share whose K, whose V has been used
+      uint32_t nqk = 0, npv = 0;      // steps so far
+      uint32_t piece = 0;
       bool ok = true;
-      // The loops over A and B are not unrolled: the instructions of all roles have to fit the
-      // instruction cache together.
-      auto issue_qk = [&](int x, uint32_t gt) {
-        const uint32_t d = tmem + kColS + 128 * x, dq = dq0 + x * kTileStep, dk = dk0 + (gt & 1) * kTileStep;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t ko = (k >> 2) * kHalfStep + (k & 3) * 2;
-          tc_mma_ss(d, dq + ko, dk + ko, kDescHi, idesc_qk, k > 0);
-        }
-        tc_commit(bar(BAR_SFULL + x));
-      };
-      auto issue_pv = [&](int x, uint32_t gt, uint32_t ph, uint32_t acc) -> bool {
-        const uint32_t pcol = tmem + kColS + 128 * x, ocol = tmem + kColO + 128 * x;
-        const uint32_t dv = dv0 + (gt & 1) * kTileStep;
-        if (!mbar_wait(bar(BAR_VFULL + (gt & 1)), (gt >> 1) & 1, abort_flag, err, 6)) return false;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) { // the first 64 positions of P are published before the others
-          if (!mbar_wait(bar(BAR_PHALF + 2 * h + x), ph, abort_flag, err, 10)) return false;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            tc_mma_ts(ocol, pcol + 32 * h + 8 * k, dv + (4 * h + k) * (2048 >> 4), kDescHi, idesc_pv, acc);
-            acc = 1u;
-          }
-        }
-        tc_commit(bar(BAR_ODONE + x));
-        return true;
-      };
-      uint32_t cnt = 0;               // bit x: parity of the P.V products issued for tile x
       do {
-        const int i0 = w.i0, i1 = w.i1, ns_tiles = w.s.ns_tiles;
-        const int fa = w.hx[0].fx, ea = w.hx[0].ex, fb = w.hx[1].fx, eb = w.hx[1].ex;
-        auto sees = [&](int x, int i) { const int e = x ? eb : ea; return e > 0 && (i < ns_tiles || (i >= (x ? fb : fa) && i < e)); };
-        uint32_t begun = 0;
-        // step i: P.V of tile i, then Q.K of tile i + 1, for A and for B
-        for (int i = i0 - 1; ok && i < i1; ++i) {
-          const bool more = i + 1 < i1;
-          const uint32_t gk = g + static_cast<uint32_t>(i + 1 - i0), gv = gk - 1;
-          if (more) ok = mbar_wait(bar(BAR_KFULL + (gk & 1)), (gk >> 1) & 1, abort_flag, err, 4);
-#pragma unroll 1
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (i < i0) { // the rows of Q; their writers have also taken the previous piece's results out
-              ok = mbar_wait(bar(BAR_QFULL + x), piece & 1, abort_flag, err, 3);
-              mbar_arrive(bar(BAR_QTAKEN + x));
-            } else if (sees(x, i)) {
-              ok = issue_pv(x, gv, (cnt >> x) & 1, (begun >> x) & 1);
-              cnt ^= 1u << x;
-              begun |= 1u << x;
+        const int i0 = __shfl_sync(0xffffffffu, w.i0, 0), i1 = __shfl_sync(0xffffffffu, w.i1, 0), ns_tiles = __shfl_sync(0xffffffffu, w.s.ns_tiles, 0);
+        const int fx = __shfl_sync(0xffffffffu, w.hx[x].fx, 0), ex = __shfl_sync(0xffffffffu, w.hx[x].ex, 0);
+        // the rows of Q; their writers have also taken the previous piece's results out
+        ok = wait(BAR_QFULL + x, piece & 1, 3);
+        if (!ok) break;
+        if (leader) mbar_arrive(ubar(BAR_QTAKEN + x));
+        uint32_t acc = 0, h = 0, ph = 0;
+        bool pending = false;          // a step whose scores have been issued, but not its P.V
+        for (int i = i0; i <= i1;) {
+          const bool more = i < i1, on = more && ex > 0 && (i < ns_tiles || (i >= fx && i < ex));
+          if (on) {                    // S = Q.K of step h
+            const uint32_t s = gk & 1;
+            if (h == 0) ok = wait(BAR_KFULL + s, (gk >> 1) & 1, 4);
+            ok = ok && wait(BAR_SFREE + x, (nqk & 1) ^ 1, 11);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t dk = dk0 + s * kTileStep + h * kRows64;
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const uint32_t ko = (k >> 2) * kHalfStep + (k & 3) * 2;
+                tc_mma_ss(scol, dq0 + ko, dk + ko, kDescHi, idesc_qk, k > 0);
+              }
+              tc_commit(ubar(BAR_SFULL + x));
+              if (h) tc_commit(ubar(BAR_KEMPTY + s)); // arrives when the products issued so far have read their operands
             }
-            if (ok && more && sees(x, i + 1)) {
-              tc_fence_after();
-              issue_qk(x, gk);
+            __syncwarp();
+            ++nqk;
+          }
+          if (pending) {               // O += P.V of the step before
+            const uint32_t s = gv & 1;
+            if (ph == 0) ok = wait(BAR_VFULL + s, (gv >> 1) & 1, 6);
+            ok = ok && wait(BAR_PFULL + 2 * ph + x, (npv >> 1) & 1, 10);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t dv = dv0 + s * kTileStep + ph * kRows64, pc = pcol + 32 * ph;
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) tc_mma_ts(ocol, pc + 8 * k, dv + k * (2048 >> 4), kDescHi, idesc_pv, k > 0 ? 1u : acc);
+              tc_commit(ubar(BAR_ODONE + 2 * ph + x));
+              if (ph) tc_commit(ubar(BAR_VEMPTY + s));
             }
+            __syncwarp();
+            acc = 1u;
+            ++npv;
+            gv += ph;
           }
-          if (!ok) break;
-          if (i >= i0) {
-            ok = mbar_wait(bar(BAR_VFULL + (gv & 1)), (gv >> 1) & 1, abort_flag, err, 6); // a stage is freed only after it was filled
-            tc_commit(bar(BAR_VEMPTY + (gv & 1)));
+          pending = on;
+          ph = h;
+          if (on) {
+            gk += h;
+            i += static_cast<int>(h);
+            h ^= 1u;
+          } else {
+            if (more) {                // a tile that X has no use for
+              ok = wait(BAR_KFULL + (gk & 1), (gk >> 1) & 1, 5) && wait(BAR_VFULL + (gv & 1), (gv >> 1) & 1, 5);
+              if (!ok) break;
+              if (leader) {
+                mbar_arrive(ubar(BAR_KEMPTY + (gk & 1)));
+                mbar_arrive(ubar(BAR_VEMPTY + (gv & 1)));
+              }
+              ++gk;
+              ++gv;
+            }
+            ++i;
           }
-          if (more) tc_commit(bar(BAR_KEMPTY + (gk & 1)));
         }
-        g += static_cast<uint32_t>(i1 - i0);
         ++piece;
-      } while (ok && w.next(cp));
+      } while (ok && next_piece(w, cp, lane));
     }
   } else if (warp < 12) {
-    reg_inc<160>();
+    reg_inc<152>();
     // ------------------------------------------------------------ softmax, Q and results of tile X
     const int x = (warp >> 2) - 1, quad = warp & 3;
     const int r = quad * 32 + lane;              // row of the tile
     const int tok = r / G, hd = r - tok * G;     // its token and head of the group
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t scol = tmem + lane_addr + kColS + 128 * x, ocol = tmem + lane_addr + kColO + 128 * x;
+    const uint32_t scol = tmem + lane_addr + kColS + 64 * x, pcol = tmem + lane_addr + kColP + 64 * x, ocol = tmem + lane_addr + kColO + 128 * x;
     uint32_t g = 0, cnt = 0;
     int piece = 0;
     bool ok = true;
@@ -486,7 +526,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       const bool live = tok < hx.n_tok;          // tok < tile_tokens for every row that exists
       const long t = static_cast<long>(w.s.t0) + x * cp.tile_tokens + tok;
       // a tile that sees nothing of a piece must not run more than one piece ahead of the MMA warp
-      if (piece > 0 && !__all_sync(0xffffffffu, mbar_wait(bar(BAR_QTAKEN + x), (piece - 1) & 1, abort_flag, err, 13))) break;
+      if (piece > 0 && !__all_sync(0xffffffffu, await(bar(BAR_QTAKEN + x), (piece - 1) & 1, abort_flag, err, 13))) break;
       // ---- the row of Q, scaled to fp16: its largest magnitude to 2^13 .. 2^14
       float rowc, up;
       {
@@ -536,83 +576,86 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 
       const int pos = hx.first + tok;
       const int vend = live ? min(pos + 1, w.s.end) : 0, wlo = window_begin(pos, p.window);
-      const int i0 = w.i0, i1 = w.i1, ns_tiles = w.s.ns_tiles;
+      const int i0 = w.i0, i1 = w.i1, ns_tiles = w.s.ns_tiles, skip = w.s.w0 - ns_tiles;
+      const int fx = hx.fx, ex = hx.ex, ga = hx.ga, gb = hx.gb, gs = hx.gs;
       float m_ref = -INFINITY, l = 0.f;
       bool begun = false;
       for (int i = i0; i < i1; ++i, ++g) {
-        if (!hx.sees(i, ns_tiles)) continue;
-        ok = ok && mbar_wait(bar(BAR_SFULL + x), cnt & 1, abort_flag, err, 7);
-        ok = ok && mbar_wait(bar(BAR_REF + (g & 3)), (g >> 2) & 1, abort_flag, err, 12); // complete by now: K was converted before S
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int rk = refs[2 * (g & 3)], rv = refs[2 * (g & 3) + 1];
-        const float a = fmaxf(rowc * pow2i(rk - 7), 1.2e-38f), off = static_cast<float>(rv - 7);
-        const bool all = hx.sees_all(i);
-        const int col0 = w.s.tile(i) * kBN;
-        // hides what the row does not see of 64 columns from column 64 h
-        auto hide = [&](uint32_t (&v)[64], int h) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int c0 = col0 + 64 * h + 32 * q;
-            auto below = [&](int k) { return k - c0 <= 0 ? 0u : k - c0 >= 32 ? 0xffffffffu : (1u << (k - c0)) - 1u; }; // columns < k
-            const uint32_t vis = below(vend) & (~below(wlo) | below(p.n_sink));
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!(vis & (1u << j))) v[32 * q + j] = 0xff800000u; // -inf
-          }
-        };
-        // The row is read twice, for its maximum and for its weights, 64 columns at a time: kept whole it
-        // would not fit the registers, and unrolled whole the instructions would not fit their cache.
-        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (!(ex > 0 && (i < ns_tiles || (i >= fx && i < ex)))) continue;
+        const bool all = i < gs || (i >= ga && i < gb);     // every row sees all of the tile
+        const int col0 = (i < ns_tiles ? i : i + skip) * kBN;
+        float a = 0.f, off = 0.f, inv_v = 0.f;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          uint32_t su[64];
-          tc_ld32(scol + 64 * h, su);
-          tc_ld32(scol + 64 * h + 32, su + 32);
-          tc_wait_ld();
-          if (!all) hide(su, h);
-#pragma unroll
-          for (int j = 0; j < 64; j += 8) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mxa[k] = max3(mxa[k], __uint_as_float(su[j + k]), __uint_as_float(su[j + 4 + k]));
-          }
-        }
-        const float mx = fmaf(fmaxf(fmaxf(mxa[0], mxa[1]), fmaxf(mxa[2], mxa[3])), a, off);
-        const bool grow = mx > m_ref + kLazy;
-        if (__any_sync(0xffffffffu, grow) && begun) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(BAR_ODONE + x), (cnt - 1) & 1, abort_flag, err, 8))) {
+        for (uint32_t h = 0; h < 2; ++h, ++cnt) {
+          ok = ok && await(bar(BAR_SFULL + x), cnt & 1, abort_flag, err, 7);
+          if (h == 0) ok = ok && await(bar(BAR_REF + (g & 3)), (g >> 2) & 1, abort_flag, err, 12); // complete by now: K was converted before S
+          // this half of P was last read by the product two steps ago: almost always done by now, asked early
+          uint32_t p_free = cnt < 2 || mbar_try_wait(bar(BAR_ODONE + 2 * h + x), ((cnt - 2) >> 1) & 1);
+          if (__builtin_expect(!__all_sync(0xffffffffu, ok), 0)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const float f = grow ? ex2(m_ref - mx) : 1.f;
-          l *= f;
-#pragma unroll 1
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t o[32];
-            tc_ld32(ocol + 32 * q4, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tc_st32(ocol + 32 * q4, o);
+          uint32_t su[64];
+          tc_ld32(scol, su);
+          tc_ld32(scol + 32, su + 32);
+          if (h == 0) {
+            const int rk = refs[2 * (g & 3)], rv = refs[2 * (g & 3) + 1];
+            a = fmaxf(rowc * pow2i(rk - 7), 1.2e-38f);
+            off = static_cast<float>(rv - 7);
+            inv_v = pow2i(7 - rv);
           }
-          tc_wait_st();
-        }
-        if (grow) m_ref = mx;
-        begun = true;
-        const float nm = off - (m_ref == -INFINITY ? 0.f : m_ref); // nothing seen yet: P = 0
-        uint64_t sums[2] = {0ull, 0ull};
-        const uint64_t a2 = pack2(a, a), nm2 = pack2(nm, nm);
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          uint32_t su[64], pk[32];
-          tc_ld32(scol + 64 * h, su);
-          tc_ld32(scol + 64 * h + 32, su + 32);
           tc_wait_ld();
-          if (!all) hide(su, h);
+          tc_fence_before();
+          mbar_arrive(bar(BAR_SFREE + x));   // the scores are in registers: the next step's may come
+          if (__builtin_expect(!all, 0)) { // hide what the row does not see
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int c0 = col0 + 64 * static_cast<int>(h) + 32 * q;
+              auto below = [&](int k) { return k - c0 <= 0 ? 0u : k - c0 >= 32 ? 0xffffffffu : (1u << (k - c0)) - 1u; }; // columns < k
+              const uint32_t vis = below(vend) & (~below(wlo) | below(p.n_sink));
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!(vis & (1u << j))) su[32 * q + j] = 0xff800000u; // -inf
+            }
+          }
+          float mxa[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mxa[k] = fmaxf(__uint_as_float(su[k]), __uint_as_float(su[8 + k]));
+#pragma unroll
+          for (int j = 16; j < 64; j += 16) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mxa[k] = max3(mxa[k], __uint_as_float(su[j + k]), __uint_as_float(su[j + 8 + k]));
+          }
+          const float mx = fmaf(fmaxf(max3(mxa[0], mxa[1], mxa[2]), max3(max3(mxa[3], mxa[4], mxa[5]), mxa[6], mxa[7])), a, off);
+          const bool grow = mx > m_ref + kLazy;
+          if (__builtin_expect(__any_sync(0xffffffffu, grow) && begun, 0)) {
+            // O must hold every product issued so far: those of this half's last step and of the other's
+            ok = await(bar(BAR_ODONE + 2 * (h ^ 1) + x), ((cnt - 1) >> 1) & 1, abort_flag, err, 8);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const float f = grow ? ex2(m_ref - mx) : 1.f;
+            l *= f;
+#pragma unroll 1
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t o[32];
+              tc_ld32(ocol + 32 * q4, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tc_st32(ocol + 32 * q4, o);
+            }
+            tc_wait_st();
+          }
+          if (grow) m_ref = mx;
+          begun = true;
+          const float nm = off - (m_ref == -INFINITY ? 0.f : m_ref); // nothing seen yet: P = 0
+          uint64_t sums[2] = {0ull, 0ull};
+          const uint64_t a2 = pack2(a, a), nm2 = pack2(nm, nm);
+          uint32_t pk[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const uint64_t y2 = fma2(pack2(__uint_as_float(su[2 * j]), __uint_as_float(su[2 * j + 1])), a2, nm2);
@@ -622,22 +665,27 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             sums[j & 1] = add2(sums[j & 1], pack2(e0, e1));
             pk[j] = Elem<__half>::pack(e0, e1);
           }
-          tc_st32(scol + 32 * h, pk); // 64 fp16 weights over columns of S that have been read
-          tc_wait_st();
-          tc_fence_before();
-          mbar_arrive(bar(BAR_PHALF + 2 * h + x));
-        }
-        {
+          if (__builtin_expect(!__all_sync(0xffffffffu, p_free), 0)) {
+            ok = await(bar(BAR_ODONE + 2 * h + x), ((cnt - 2) >> 1) & 1, abort_flag, err, 14);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+          }
+          tc_st32(pcol + 32 * h, pk);
           float s0, s1, s2, s3;
           unpack2(sums[0], s0, s1);
           unpack2(sums[1], s2, s3);
-          l = fmaf((s0 + s1) + (s2 + s3), pow2i(7 - rv), l);
+          l = fmaf((s0 + s1) + (s2 + s3), inv_v, l);
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(BAR_PFULL + 2 * h + x));
         }
-        ++cnt;
+        if (!ok) break;
       }
       if (!ok) break;
       // ---- the piece's result
-      if (begun && !__all_sync(0xffffffffu, mbar_wait(bar(BAR_ODONE + x), (cnt - 1) & 1, abort_flag, err, 9))) {
+      if (begun && !__all_sync(0xffffffffu, await(bar(BAR_ODONE + 2 + x), ((cnt - 1) >> 1) & 1, abort_flag, err, 9))) {
         ok = false;
         break;
       }
@@ -679,44 +727,45 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       ++piece;
     } while (next_piece(w, cp, lane));
   } else {
-    reg_dec<96>();
+    reg_dec<112>();
     // ------------------------------------------------------------ converters: 32 rows of every tile per warp
     const int cw = warp - 12;
     uint32_t g = 0;
     bool ok = true;
-    // rows 32 cw .. 32 cw + 31 of the raw tile -> fp16 operand tile; `f`: this lane's row's factor, two fp16 (0: zeros)
+    // Rows 32 cw .. 32 cw + 31 of the raw tile -> fp16 operand tile.  `f`: this lane's row's factor, two
+    // fp16 (0: a row that nobody sees, written as zeros).  Eight lanes access shared memory at once: four
+    // 16-byte pieces of the codes of row a and of row a ^ 5, which the 128-byte swizzle of the codes puts
+    // into eight different bank groups, and that of the operand tile as well.
+    const int pr = (lane >> 3) ^ ((lane & 4) ? 5 : 0);
     auto convert = [&](uint32_t raw, uint32_t dst, uint32_t f) {
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        uint32_t wv[4][4]; // sixteen rows are under way at once
+      const bool hole = __any_sync(0xffffffffu, f == 0u);
+      uint32_t wv[8][4], fr[4];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const int row = 32 * cw + half * 16 + it * 4 + (lane >> 3);
+      for (int b8 = 0; b8 < 4; ++b8) {       // eight rows, both 64-element halves
+        const int rl = b8 * 8 + pr, row = 32 * cw + rl, sw = row & 7;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(wv[it][0]), "=r"(wv[it][1]), "=r"(wv[it][2]), "=r"(wv[it][3])
-                       : "r"(raw + row * 128 + (lane & 7) * 16));
-        }
+                       : "=r"(wv[2 * b8 + h][0]), "=r"(wv[2 * b8 + h][1]), "=r"(wv[2 * b8 + h][2]), "=r"(wv[2 * b8 + h][3])
+                       : "r"(raw + row * 128 + (((4 * h + (lane & 3)) ^ sw) << 4)));
+        fr[b8] = __shfl_sync(0xffffffffu, f, rl);
+      }
+      if (__builtin_expect(hole, 0)) {
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const int rl = half * 16 + it * 4 + (lane >> 3), row = 32 * cw + rl, ch = lane & 7; // elements 16 ch ..
-          const uint32_t fr = __shfl_sync(0xffffffffu, f, rl);
-          uint32_t h[8];
+        for (int e = 0; e < 32; ++e)
+          if (fr[e >> 3] == 0u) wv[e >> 2][e & 3] = 0u; // whatever the bytes are
+      }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t v = hmul2(cvt_e4m3x2_f16x2((wv[it][e >> 1] >> (16 * (e & 1))) & 0xffffu), fr);
-            h[e] = fr ? v : 0u;
-          }
-          // two 16-byte chunks of the row's half tile; lanes of the two halves write them in opposite order
-          // (the halves lie 16 KB apart, in the same banks)
-          const uint32_t base = dst + (ch >> 2) * kHalfTile + row * 128, c0 = 2 * (ch & 3), flip = ch >> 2;
+      for (int b8 = 0; b8 < 4; ++b8) {
+        const int row = 32 * cw + b8 * 8 + pr, sw = row & 7;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t q = k ^ flip;
-            const uint32_t at = base + (((c0 + q) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q ? h[4] : h[0]), "r"(q ? h[5] : h[1]), "r"(q ? h[6] : h[2]),
-                         "r"(q ? h[7] : h[3])
-                         : "memory");
-          }
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = hmul2(cvt_e4m3x2_f16x2((wv[2 * b8 + h][e >> 1] >> (16 * (e & 1))) & 0xffffu), fr[b8]);
+          const uint32_t base = dst + h * kHalfTile + row * 128, c0 = 2 * (lane & 3);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + ((c0 ^ sw) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (((c0 + 1) ^ sw) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
         }
       }
     };
@@ -729,7 +778,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       for (int i = w.i0; ok && i < w.i1; ++i, ++g) {
         const int col0 = w.s.tile(i) * kBN;
         const uint32_t ph = g & 1, s = g & 1, sph = (g >> 1) & 1;
-        ok = mbar_wait(bar(BAR_RAWFULL + 0), ph, abort_flag, err, 20);
+        ok = await(bar(BAR_RAWFULL + 0), ph, abort_flag, err, 20);
         if (!__all_sync(0xffffffffu, ok)) break;
         // the largest exponents among the rows that someone sees (every warp for itself: 4 rows a lane)
         const uint32_t kx4 = *reinterpret_cast<const uint32_t *>(smem + kSmemExp + 4 * lane);
@@ -750,8 +799,8 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const uint32_t fv = !vis || poison ? 0u : factor(rv - vx);
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
-          if (kv) ok = mbar_wait(bar(BAR_RAWFULL + 1), ph, abort_flag, err, 22);
-          ok = ok && mbar_wait(bar((kv ? BAR_VEMPTY : BAR_KEMPTY) + s), sph ^ 1, abort_flag, err, 21);
+          if (kv) ok = await(bar(BAR_RAWFULL + 1), ph, abort_flag, err, 22);
+          ok = ok && await(bar((kv ? BAR_VEMPTY : BAR_KEMPTY) + s), sph ^ 1, abort_flag, err, 21);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -879,8 +928,8 @@ cudaError_t launch_attn_q8_chunk(const Q8AttnParams &p, bool bf16, cudaStream_t 
   const uint64_t rows = c.pg.table ? 1ull << c.pg.page_shift : static_cast<uint64_t>(c.max_pos);
   const uint64_t outers = c.pg.table ? static_cast<uint64_t>(c.pg.n_pages) : static_cast<uint64_t>(c.batch);
   CUtensorMap mk, mv;
-  if (!make_tensor_map_u8(&mk, false, c.k, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64) ||
-      !make_tensor_map_u8(&mv, false, c.v, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64))
+  if (!make_tensor_map_u8(&mk, true, c.k, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64) ||
+      !make_tensor_map_u8(&mv, true, c.v, rows, c.n_kv_heads, outers, c.c_pos, c.c_head, c.c_outer, 64))
     return cudaErrorNotSupported;
   return bf16 ? launch_typed<__nv_bfloat16>(cp, mk, mv, n_ctas, blocks, stream, launches)
               : launch_typed<__half>(cp, mk, mv, n_ctas, blocks, stream, launches);
