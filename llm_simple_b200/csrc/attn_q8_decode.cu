@@ -6,11 +6,13 @@
 // and every CTA takes an equal, contiguous share of that line.  The lengths are read on the device:
 // each CTA adds up the runs of the batch (a scan of `batch` integers, about a microsecond) and finds
 // its share, so a captured graph follows the lengths.  Six warps:
-//   warps 0-3  16 of a tile's 64 positions each: S = Q K^T and O += P V as mma.sync m16n8k16 on fp16.
-//              e4m3 converts to fp16 exactly, two codes an instruction, straight from the bytes of
-//              the tile: a lane's share of a K row is 32 consecutive bytes (the order of the 128
-//              elements in the contraction is free, as long as Q's is the same), and its share of V
-//              is 16 consecutive bytes of four rows, whose bytes two permutes pair up.
+//   warps 0-3  32 positions of every other tile each: S^T = K Q^T and O^T += V^T P^T as mma.sync
+//              m16n8k16 on fp16 -- positions and elements fill the M dimension, the few query rows
+//              the N dimension of 8 (up to 16: two of them).  e4m3 converts to fp16 exactly, two codes
+//              an instruction, straight from the bytes of the tile: a lane's share of a K row is 32
+//              consecutive bytes (the order of the 128 elements in the contraction is free, as long
+//              as Q's is the same), and its share of V is 16 consecutive bytes of four rows, whose
+//              bytes two permutes pair up.
 //   warp 4     TMA producer: K and V tiles (128-byte swizzle) and their exponent bytes, 5 stages of
 //              16 KB
 //   warp 5     the piece's query rows, as fp16 scaled by a power of two (exact for bf16 and fp16)
@@ -126,7 +128,7 @@ struct Q8DecodeParams {
   int min_tiles;  // smallest share worth a CTA
 };
 
-template <typename T, bool WIDE> // WIDE: more than 8 rows
+template <typename T, int NH> // NH: query rows in eights
 __global__ void __launch_bounds__(q8d::kThreads, 2)
 attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ CUtensorMap map_k16, const __grid_constant__ CUtensorMap map_v16, const Q8DecodeParams dp) {
@@ -147,7 +149,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     prefetch_tensormap(&map_v);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar(BAR_FULL + s), 1);
-      mbar_init(bar(BAR_EMPTY + s), kConsumerWarps);
+      mbar_init(bar(BAR_EMPTY + s), 2);
     }
     mbar_init(bar(BAR_QREADY), 1);
     mbar_init(bar(BAR_QFREE), kConsumerWarps);
@@ -268,7 +270,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       if (!__all_sync(0xffffffffu, wait_ok)) return;
       const int nrows = w.s.nq * G;
 #pragma unroll
-      for (int it4 = 0; it4 < (WIDE ? 4 : 2); ++it4) {
+      for (int it4 = 0; it4 < 2 * NH; ++it4) {
         const int rho = it4 * 4 + (lane >> 3), j = lane & 7; // eight lanes per row, 16 elements each
         uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
         if (rho < nrows) {
@@ -308,6 +310,9 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   }
 
   // -------------------------------------------------------------------- consumers
+  // Fragments: rows of K are the M dimension, query rows (8 per NH) the N dimension, so that few query
+  // rows cost few products and accumulators.  This lane: positions g0 and g0 + 8 of a group of 16,
+  // query rows 2 cq and 2 cq + 1 of S; elements 16 g0 + x of O for the same query rows.
   const int g0 = lane >> 2, cq = lane & 3;
   const float kNegInf = -INFINITY, kNan = __int_as_float(0x7fc00000);
   Walk w;
@@ -318,165 +323,176 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   do {
     ok = ok && mbar_wait(bar(BAR_QREADY), it & 1, abort_flag, p.c.error_flag, 33);
     // contraction order: k-step ks of this lane covers elements 32 cq + 4 ks + {0, 1} and + {2, 3}
-    uint32_t qa[8][4];
-    float qs0, qs1 = 0.f;
-    {
-      const uint4 *r0 = reinterpret_cast<const uint4 *>(smem + kOffQ + g0 * 256 + cq * 64);
-      const uint4 *r1 = reinterpret_cast<const uint4 *>(smem + kOffQ + (g0 + 8) * 256 + cq * 64);
+    uint32_t qb[NH][8][2];
+    float qs[NH][2];
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) {
+      const uint4 *r = reinterpret_cast<const uint4 *>(smem + kOffQ + (8 * nh + g0) * 256 + cq * 64);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const uint4 a = r0[x];
-        const uint4 b = WIDE ? r1[x] : make_uint4(0, 0, 0, 0);
-        qa[2 * x][0] = a.x, qa[2 * x][2] = a.y, qa[2 * x + 1][0] = a.z, qa[2 * x + 1][2] = a.w;
-        qa[2 * x][1] = b.x, qa[2 * x][3] = b.y, qa[2 * x + 1][1] = b.z, qa[2 * x + 1][3] = b.w;
+        const uint4 v = r[x];
+        qb[nh][2 * x][0] = v.x, qb[nh][2 * x][1] = v.y, qb[nh][2 * x + 1][0] = v.z, qb[nh][2 * x + 1][1] = v.w;
       }
-      const float *qs = reinterpret_cast<const float *>(smem + kOffQs);
-      qs0 = qs[g0];
-      if (WIDE) qs1 = qs[g0 + 8];
+      const float2 s2 = *reinterpret_cast<const float2 *>(smem + kOffQs + (8 * nh + 2 * cq) * 4);
+      qs[nh][0] = s2.x, qs[nh][1] = s2.y;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(BAR_QFREE));
 
     const int nrows = w.s.nq * G;
-    const int p0 = w.s.pos0 + g0 / G, p1 = w.s.pos0 + (g0 + 8) / G; // positions of this lane's rows
-    const int end0 = min(p0 + 1, w.s.end), end1 = min(p1 + 1, w.s.end);
-    const int lo0 = window_begin(p0, p.window), lo1 = window_begin(p1, p.window);
-    // every row sees all of a tile that ends before the first row's position and begins at or behind
-    // the last row's window, or lies among the first positions
+    // every row sees all of what ends before the first row's position and begins at or behind the last
+    // row's window, or lies among the first positions
     const int all_end = min(w.s.pos0 + 1, w.s.end), all_lo = window_begin(w.s.pos0 + w.s.nq - 1, p.window);
 
-    float o[16][4];
+    float o[NH][8][4];
+    float m[NH][2], l[NH][2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = kNegInf, m1 = kNegInf, l0 = 0.f, l1 = 0.f;
+    for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) o[nh][x][0] = o[nh][x][1] = o[nh][x][2] = o[nh][x][3] = 0.f;
+      m[nh][0] = m[nh][1] = kNegInf;
+      l[nh][0] = l[nh][1] = 0.f;
+    }
 
+    // a tile is the work of two warps, 32 positions (two groups of 16) each; the other two have the next
     for (int i = w.i0; i < w.i1; ++i, ++g) {
+      if ((g & 1) != static_cast<uint32_t>(warp >> 1)) continue;
       const int s = g % kStages;
-      const int tpos = w.s.tile(i) * kTileN, col0 = tpos + warp * 16;
-      const bool some = col0 < w.s.end && (col0 + 15 >= w.s.lo || col0 < w.s.ns);
-      const bool all = tpos + kTileN <= all_end && (tpos >= all_lo || tpos + kTileN <= p.n_sink);
+      const int row0 = (warp & 1) * 32, col0 = w.s.tile(i) * kTileN + row0;
+      const bool some = col0 < w.s.end && (col0 + 31 >= w.s.lo || col0 < w.s.ns);
+      const bool all = col0 + 32 <= all_end && (col0 >= all_lo || col0 + 32 <= p.n_sink);
       ok = ok && mbar_wait(bar(BAR_FULL + s), (g / kStages) & 1, abort_flag, p.c.error_flag, 34);
       if (__all_sync(0xffffffffu, ok) && some) {
-        const uint32_t st_k = smem_base + s * kStageBytes, st_v = st_k + kTile;
-        const unsigned char *ex = smem + kOffExp + s * 128 + warp * 16;
-        float sc[2][4];
+        const uint32_t st_k = smem_base + s * kStageBytes + row0 * 128, st_v = st_k + kTile;
+        const unsigned char *ex = smem + kOffExp + s * 128 + row0;
+        float sc[2][NH][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-          const uint32_t row = st_k + (warp * 16 + nt * 8 + g0) * 128;
-          uint32_t kw[8];
+        for (int u = 0; u < 2; ++u) {
+          uint32_t kw[2][8];
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(kw[4 * x]), "=r"(kw[4 * x + 1]), "=r"(kw[4 * x + 2]), "=r"(kw[4 * x + 3])
-                         : "r"(row + (((2 * cq + x) ^ g0) << 4)));
+          for (int rr = 0; rr < 2; ++rr)
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            mma_16816<__half>(sc[nt], qa[ks], cvt_e4m3x2_f16x2(kw[ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[ks] >> 16));
+            for (int x = 0; x < 2; ++x)
+              lds128(kw[rr] + 4 * x, st_k + (16 * u + 8 * rr + g0) * 128 + (((2 * cq + x) ^ g0) << 4));
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) sc[u][nh][0] = sc[u][nh][1] = sc[u][nh][2] = sc[u][nh][3] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t ka[4] = {cvt_e4m3x2_f16x2(kw[0][ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[1][ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[0][ks] >> 16),
+                                    cvt_e4m3x2_f16x2(kw[1][ks] >> 16)};
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh) mma_16816<__half>(sc[u][nh], ka, qb[nh][ks][0], qb[nh][ks][1]);
+          }
         }
-        // exponents of this lane's four positions, two per n-tile
-        float vinv[4];
-        float tmax0 = kNegInf, tmax1 = kNegInf;
+        // V: 16 bytes (elements 16 g0 ..) of rows 2 cq + {0, 1, 8, 9} of either group
+        uint32_t vw[2][4][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const uint32_t kx2 = *reinterpret_cast<const uint16_t *>(ex + nt * 8 + 2 * cq);
-          const uint32_t vx2 = *reinterpret_cast<const uint16_t *>(ex + 64 + nt * 8 + 2 * cq);
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t kx = (kx2 >> (8 * e)) & 0xffu, vx = (vx2 >> (8 * e)) & 0xffu;
+          for (int x = 0; x < 4; ++x) {
+            const int r = 2 * cq + (x & 1) + (x >> 1) * 8;
+            lds128(vw[u][x], st_v + (16 * u + r) * 128 + ((g0 ^ (r & 7)) << 4));
+          }
+        // t = S 2^e_k scale + e_v; exponents of this lane's four positions
+        float vinv[2][2], top[NH][2];
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) top[nh][0] = top[nh][1] = kNegInf;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr) {
+            const uint32_t kx = ex[16 * u + 8 * rr + g0], vx = ex[64 + 16 * u + 8 * rr + g0];
             const float kf = (kx == kPoison || vx == kPoison) ? kNan : __uint_as_float(kx << 23);
             const float ev = static_cast<float>(static_cast<int>(vx) - 127);
-            vinv[nt * 2 + e] = __uint_as_float((254u - min(vx, 253u)) << 23);
-            float t0 = fmaf(sc[nt][e], qs0 * kf, ev);
-            float t1 = WIDE ? fmaf(sc[nt][2 + e], qs1 * kf, ev) : 0.f;
-            if (!all) {
-              const int j = col0 + nt * 8 + 2 * cq + e;
-              if (!(j < end0 && (j >= lo0 || j < p.n_sink))) t0 = kNegInf;
-              if (WIDE && !(j < end1 && (j >= lo1 || j < p.n_sink))) t1 = kNegInf;
+            vinv[u][rr] = __uint_as_float((254u - min(vx, 253u)) << 23);
+#pragma unroll
+            for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float &t = sc[u][nh][2 * rr + e];
+                t = fmaf(t, qs[nh][e] * kf, ev);
+                if (!all) {
+                  const int j = col0 + 16 * u + 8 * rr + g0, pr = w.s.pos0 + (8 * nh + 2 * cq + e) / G;
+                  if (!(j < min(pr + 1, w.s.end) && (j >= window_begin(pr, p.window) || j < p.n_sink))) t = kNegInf;
+                }
+                top[nh][e] = fmaxf(top[nh][e], t);
+              }
+          }
+        bool grow = false;
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top[nh][e] = fmaxf(top[nh][e], __shfl_xor_sync(0xffffffffu, top[nh][e], d));
+            grow |= top[nh][e] > m[nh][e] + kLazy;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const bool up = top[nh][e] > m[nh][e] + kLazy;
+              const float f = up ? tc5::ex2(m[nh][e] - top[nh][e]) : 1.f;
+              if (up) m[nh][e] = top[nh][e];
+              l[nh][e] *= f;
+#pragma unroll
+              for (int x = 0; x < 8; ++x) o[nh][x][e] *= f, o[nh][x][2 + e] *= f;
             }
-            sc[nt][e] = t0;
-            tmax0 = fmaxf(tmax0, t0);
-            if (WIDE) {
-              sc[nt][2 + e] = t1;
-              tmax1 = fmaxf(tmax1, t1);
+        }
+        // P, its 8 x 8 blocks turned so that a lane holds two positions of query row g0
+        uint32_t pb[2][NH][2];
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+          const float ms0 = m[nh][0] == kNegInf ? 0.f : m[nh][0], ms1 = m[nh][1] == kNegInf ? 0.f : m[nh][1]; // nothing seen yet: P = 0
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              const float p0 = tc5::ex2(sc[u][nh][2 * rr] - ms0), p1 = tc5::ex2(sc[u][nh][2 * rr + 1] - ms1);
+              l[nh][0] = fmaf(p0, vinv[u][rr], l[nh][0]);
+              l[nh][1] = fmaf(p1, vinv[u][rr], l[nh][1]);
+              pb[u][nh][rr] = transpose8x8(Elem<__half>::pack(p0, p1));
             }
-          }
         }
-        tmax0 = fmaxf(tmax0, __shfl_xor_sync(0xffffffffu, tmax0, 1));
-        tmax0 = fmaxf(tmax0, __shfl_xor_sync(0xffffffffu, tmax0, 2));
-        if (WIDE) {
-          tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 1));
-          tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 2));
-        }
-        const bool grow0 = tmax0 > m0 + kLazy, grow1 = WIDE && tmax1 > m1 + kLazy;
-        if (__any_sync(0xffffffffu, grow0 || grow1)) {
-          const float f0 = grow0 ? tc5::ex2(m0 - tmax0) : 1.f, f1 = grow1 ? tc5::ex2(m1 - tmax1) : 1.f;
-          if (grow0) m0 = tmax0;
-          if (grow1) m1 = tmax1;
-          l0 *= f0, l1 *= f1;
+        if (!all) {
+          // a row nobody sees may hold anything: a zero weight must not meet a NaN code
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            o[x][0] *= f0, o[x][1] *= f0;
-            if (WIDE) o[x][2] *= f1, o[x][3] *= f1;
-          }
-        }
-        const float ms0 = m0 == kNegInf ? 0.f : m0, ms1 = m1 == kNegInf ? 0.f : m1; // nothing seen yet: P = 0
-        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const float a = tc5::ex2(sc[nt][0] - ms0), b = tc5::ex2(sc[nt][1] - ms0);
-          l0 = fmaf(a, vinv[2 * nt], l0);
-          l0 = fmaf(b, vinv[2 * nt + 1], l0);
-          pa[2 * nt] = Elem<__half>::pack(a, b);
-          if (WIDE) {
-            const float c2 = tc5::ex2(sc[nt][2] - ms1), d2 = tc5::ex2(sc[nt][3] - ms1);
-            l1 = fmaf(c2, vinv[2 * nt], l1);
-            l1 = fmaf(d2, vinv[2 * nt + 1], l1);
-            pa[2 * nt + 1] = Elem<__half>::pack(c2, d2);
-          }
-        }
-        // V: 16 bytes (elements 16 g0 ..) of rows 2 cq + {0, 1, 8, 9}
-        uint32_t vw[4][4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = 2 * cq + (x & 1) + (x >> 1) * 8; // row within the warp's 16
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(vw[x][0]), "=r"(vw[x][1]), "=r"(vw[x][2]), "=r"(vw[x][3])
-                       : "r"(st_v + (warp * 16 + r) * 128 + ((g0 ^ (r & 7)) << 4)));
-          if (!all) {
-            // a row nobody sees may hold anything: a zero weight must not meet a NaN code
-            const int j = col0 + r;
-            if (!(j < w.s.end && (j >= w.s.lo || j < w.s.ns))) vw[x][0] = vw[x][1] = vw[x][2] = vw[x][3] = 0u;
-          }
+            for (int x = 0; x < 4; ++x) {
+              const int j = col0 + 16 * u + 2 * cq + (x & 1) + (x >> 1) * 8;
+              if (!(j < w.s.end && (j >= w.s.lo || j < w.s.ns))) vw[u][x][0] = vw[u][x][1] = vw[u][x][2] = vw[u][x][3] = 0u;
+            }
         }
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const uint32_t lo2 = __byte_perm(vw[0][q4], vw[1][q4], hh ? 0x7362 : 0x5140);
-            const uint32_t hi2 = __byte_perm(vw[2][q4], vw[3][q4], hh ? 0x7362 : 0x5140);
-            const int x = 4 * q4 + 2 * hh;
-            mma_16816<__half>(o[x], pa, cvt_e4m3x2_f16x2(lo2 & 0xffffu), cvt_e4m3x2_f16x2(hi2 & 0xffffu));
-            mma_16816<__half>(o[x + 1], pa, cvt_e4m3x2_f16x2(lo2 >> 16), cvt_e4m3x2_f16x2(hi2 >> 16));
-          }
-        }
+          for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              const uint32_t lo2 = __byte_perm(vw[u][0][q4], vw[u][1][q4], hh ? 0x7362 : 0x5140);
+              const uint32_t hi2 = __byte_perm(vw[u][2][q4], vw[u][3][q4], hh ? 0x7362 : 0x5140);
+              const uint32_t va[4] = {cvt_e4m3x2_f16x2(lo2 & 0xffffu), cvt_e4m3x2_f16x2(lo2 >> 16), cvt_e4m3x2_f16x2(hi2 & 0xffffu),
+                                      cvt_e4m3x2_f16x2(hi2 >> 16)};
+#pragma unroll
+              for (int nh = 0; nh < NH; ++nh) mma_16816<__half>(o[nh][2 * q4 + hh], va, pb[u][nh][0], pb[u][nh][1]);
+            }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(BAR_EMPTY + s));
     }
 
     // ---- the four warps' states of the piece -> its result.  Accumulator x of a lane holds elements
-    //      32 cq + x and 32 cq + 16 + x of its rows.
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (cq == 0) {
-      red_ml[(warp * 16 + g0) * 2] = m0;
-      red_ml[(warp * 16 + g0) * 2 + 1] = l0;
-      red_ml[(warp * 16 + g0 + 8) * 2] = m1;
-      red_ml[(warp * 16 + g0 + 8) * 2 + 1] = l1;
-    }
+    //      16 g0 + 2 x and 16 g0 + 2 x + 1 of its two query rows.
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nh][e] += __shfl_xor_sync(0xffffffffu, l[nh][e], d);
+        if (g0 == 0) *reinterpret_cast<float2 *>(red_ml + (warp * 16 + 8 * nh + 2 * cq + e) * 2) = make_float2(m[nh][e], l[nh][e]);
+      }
     consumer_sync();
     auto row_ml = [&](int row, float &M, float &L) {
       M = kNegInf;
@@ -491,36 +507,35 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int slot = 2 * c + (it == 0 ? 0 : 1);
     float *buf = reinterpret_cast<float *>(smem + kOffCombine);
 #pragma unroll
-    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
-      if (half * 8 < nrows) {
-        float M, L;
-        row_ml(g0 + 8 * half, M, L);
-        const float mw = half ? m1 : m0;
-        // L is NaN where a poisoned row was seen, and 0 where nothing was
-        const float f = L == 0.f ? 0.f : exp2f(mw - (M == kNegInf ? 0.f : M)) / L;
+    for (int nh = 0; nh < NH; ++nh) {
+      if (nh * 8 < nrows) {
 #pragma unroll
-        for (int q8i = 0; q8i < 8; ++q8i) {
-          // chunk of four elements 32 cq + 4 q8i, its place turned by lane so that eight lanes hit eight banks
-          const int hi = q8i >> 2, x = (q8i & 3) * 4, e = 2 * half + hi;
-          const float4 v = make_float4(o[x][e] * f, o[x + 1][e] * f, o[x + 2][e] * f, o[x + 3][e] * f);
-          const int chunk = 8 * cq + (q8i ^ ((2 * cq + (g0 & 1)) & 7));
-          reinterpret_cast<float4 *>(buf)[(warp * 8 + g0) * 32 + chunk] = v;
+        for (int e = 0; e < 2; ++e) {
+          float M, L;
+          row_ml(8 * nh + 2 * cq + e, M, L);
+          // L is NaN where a poisoned row was seen, and 0 where nothing was
+          const float f = L == 0.f ? 0.f : exp2f(m[nh][e] - (M == kNegInf ? 0.f : M)) / L;
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            // four elements 16 g0 + 4 q4, their place turned by the row so that eight lanes hit eight banks
+            const float4 v = make_float4(o[nh][2 * q4][e] * f, o[nh][2 * q4][2 + e] * f, o[nh][2 * q4 + 1][e] * f, o[nh][2 * q4 + 1][2 + e] * f);
+            reinterpret_cast<float4 *>(buf)[(warp * 8 + 2 * cq + e) * 32 + ((4 * g0 + q4) ^ cq)] = v;
+          }
         }
       }
       consumer_sync();
-      const int rr = tid >> 4, rho = rr + 8 * half;
+      const int rr = tid >> 4, rho = rr + 8 * nh;
       if (rho < nrows) {
         const int tok = rho / G;
         const long t = w.s.t0 + tok;
         const int h = w.kvh * G + rho - tok * G;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int ch = (tid & 15) + 16 * k, cc = ch >> 3;
-          const int chunk = 8 * cc + ((ch & 7) ^ ((2 * cc + (rr & 1)) & 7));
+          const int ch = (tid & 15) + 16 * k;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int x = 0; x < kConsumerWarps; ++x) {
-            const float4 u = reinterpret_cast<const float4 *>(buf)[(x * 8 + rr) * 32 + chunk];
+            const float4 u = reinterpret_cast<const float4 *>(buf)[(x * 8 + rr) * 32 + (ch ^ (rr >> 1))];
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
           }
           if (whole) {
@@ -612,23 +627,23 @@ template <typename T> __global__ void __launch_bounds__(128) attn_q8_merge_kerne
 namespace {
 
 // the shared-memory opt-in is a property of (function, device): set on the first launch per device
-template <typename T, bool WIDE> cudaError_t opt_in() {
+template <typename T, int NH> cudaError_t opt_in() {
   static bool done[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || !done[dev]) {
-    e = cudaFuncSetAttribute(attn_q8_decode_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, q8d::kSmemTotal);
+    e = cudaFuncSetAttribute(attn_q8_decode_kernel<T, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, q8d::kSmemTotal);
     if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
   }
   return e;
 }
 
-template <typename T, bool WIDE>
+template <typename T, int NH>
 cudaError_t launch_typed(const Q8DecodeParams &dp, int n_ctas, const CUtensorMap *m, cudaStream_t stream, int *launches) {
-  cudaError_t e = opt_in<T, WIDE>();
+  cudaError_t e = opt_in<T, NH>();
   if (e != cudaSuccess) return e;
-  e = launch_dependent(attn_q8_decode_kernel<T, WIDE>, dim3(n_ctas), q8d::kThreads, q8d::kSmemTotal, stream, m[0], m[1], m[2], m[3], dp);
+  e = launch_dependent(attn_q8_decode_kernel<T, NH>, dim3(n_ctas), q8d::kThreads, q8d::kSmemTotal, stream, m[0], m[1], m[2], m[3], dp);
   if (e != cudaSuccess) return e;
   *launches = 1;
   e = launch_dependent(attn_q8_merge_kernel<T>, dim3(dp.a.c.batch * dp.a.c.n_kv_heads, dp.rows), 128, 0, stream, dp);
@@ -672,8 +687,8 @@ cudaError_t launch_attn_q8_decode(const Q8AttnParams &p, bool bf16, cudaStream_t
       return cudaErrorNotSupported;
   const bool wide = dp.rows > 8;
   if (bf16)
-    return wide ? launch_typed<__nv_bfloat16, true>(dp, n_ctas, m, stream, launches) : launch_typed<__nv_bfloat16, false>(dp, n_ctas, m, stream, launches);
-  return wide ? launch_typed<__half, true>(dp, n_ctas, m, stream, launches) : launch_typed<__half, false>(dp, n_ctas, m, stream, launches);
+    return wide ? launch_typed<__nv_bfloat16, 2>(dp, n_ctas, m, stream, launches) : launch_typed<__nv_bfloat16, 1>(dp, n_ctas, m, stream, launches);
+  return wide ? launch_typed<__half, 2>(dp, n_ctas, m, stream, launches) : launch_typed<__half, 1>(dp, n_ctas, m, stream, launches);
 }
 
 } // namespace b200attn
