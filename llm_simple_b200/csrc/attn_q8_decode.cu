@@ -13,7 +13,7 @@
 //              consecutive bytes (the order of the 128 elements in the contraction is free, as long
 //              as Q's is the same), and its share of V is 16 consecutive bytes of four rows, whose
 //              bytes two permutes pair up.
-//   warp 4     TMA producer: K and V tiles (128-byte swizzle) and their exponent bytes, 5 stages of
+//   warp 4     TMA producer: K and V tiles (128-byte swizzle) and their exponent bytes, 4 stages of
 //              16 KB
 //   warp 5     the piece's query rows, as fp16 scaled by a power of two (exact for bf16 and fp16)
 // The row exponents never touch the products.  With e_k, e_v those of a position,
@@ -39,7 +39,11 @@ using namespace tma;
 constexpr int kConsumerWarps = 4;
 constexpr int kConsumerThreads = kConsumerWarps * 32;
 constexpr int kThreads = kConsumerThreads + 64;
-constexpr int kStages = 5;
+constexpr int kStages = 4;
+// Tile g of a share lies in stage g % kStages and belongs to consumer pair g % 2.  With an even number of
+// stages a pair sees every phase of its stages' barriers; with an odd one it would see every other, and a
+// wait on a phase's parity could not tell a phase from the one two before.
+static_assert(kStages % 2 == 0, "stages are owned by consumer pairs");
 constexpr int kTileN = 64;
 constexpr uint32_t kTile = kTileN * 128;             // K or V codes of a tile
 constexpr uint32_t kStageBytes = 2 * kTile;
@@ -53,6 +57,7 @@ constexpr uint32_t kOffBar = kOffScan + 64;
 constexpr uint32_t kSmemTotal = kOffBar + 128;
 static_assert(kSmemTotal <= 115712, "two CTAs per SM");
 constexpr int kMaxCtas = 296;                        // two per SM
+constexpr int kPieceCost = 4;                        // what a run costs besides its tiles, in tiles
 constexpr float kLazy = 8.0f;                        // log2 of how far P may exceed 1 before O is rescaled
 
 enum { BAR_FULL = 0, BAR_EMPTY = kStages, BAR_QREADY = 2 * kStages, BAR_QFREE, BAR_COUNT };
@@ -84,16 +89,21 @@ struct Walk {
   int b, kvh, i0, i1;
   long left;
   Seq s;
-  __device__ __forceinline__ void begin(const Q8AttnParams &p, int b_, long offset, long tiles) {
+  // `offset`: the share's begin on the runs of sequence b; a run is kPieceCost, then its tiles.  False: the
+  // share is all cost and no tile.
+  __device__ __forceinline__ bool begin(const Q8AttnParams &p, int b_, long offset, long share) {
     b = b_;
     s = seq_of(p, b);
-    kvh = static_cast<int>(offset / s.n_tiles);
-    i0 = static_cast<int>(offset - static_cast<long>(kvh) * s.n_tiles);
-    left = tiles;
+    const int one = s.n_tiles + kPieceCost;
+    kvh = static_cast<int>(offset / one);
+    const int at = static_cast<int>(offset - static_cast<long>(kvh) * one);
+    i0 = max(0, at - kPieceCost);
+    left = share - max(0, kPieceCost - at);
     i1 = static_cast<int>(min(static_cast<long>(s.n_tiles), i0 + left));
+    return left > 0;
   }
   __device__ __forceinline__ bool next(const Q8AttnParams &p) { // false: the share is done
-    left -= i1 - i0;
+    left -= i1 - i0 + kPieceCost;
     if (left <= 0) return false;
     if (++kvh == p.c.n_kv_heads) {
       kvh = 0;
@@ -107,6 +117,7 @@ struct Walk {
     return true;
   }
 };
+__device__ __forceinline__ int run_cost(const Seq &s) { return s.n_tiles > 0 ? s.n_tiles + kPieceCost : 0; }
 
 // A piece's partial goes to slot 2 c (the share's first piece) or 2 c + 1 (its last one).  Which slots
 // a cut run left: first and last CTA, and the slot of the first; of the others it is 2 c.
@@ -162,7 +173,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int per = (p.c.batch + kThreads - 1) / kThreads;
   const int b_lo = min(p.c.batch, tid * per), b_hi = min(p.c.batch, b_lo + per);
   int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += seq_of(p, b).n_tiles;
+  for (int b = b_lo; b < b_hi; ++b) mine += run_cost(seq_of(p, b));
   int incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -187,7 +198,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (x0 >= static_cast<long>(before) * kvH && x0 < static_cast<long>(before + mine) * kvH) {
     long at = static_cast<long>(before) * kvH;
     for (int b = b_lo; b < b_hi; ++b) {
-      const long run = static_cast<long>(seq_of(p, b).n_tiles) * kvH;
+      const long run = static_cast<long>(run_cost(seq_of(p, b))) * kvH;
       if (x0 < at + run) {
         scan[8] = b;
         scan[9] = static_cast<int>(x0 - at);
@@ -202,7 +213,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (warp == kConsumerWarps) {
     // ------------------------------------------------------------------ TMA producer
     Walk w;
-    w.begin(p, b_first, off_first, x1 - x0);
+    if (!w.begin(p, b_first, off_first, x1 - x0)) return;
     uint32_t g = 0;
     do {
       for (int base = w.i0; base < w.i1; base += 32) {
@@ -261,7 +272,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   if (warp == kConsumerWarps + 1) {
     // ------------------------------------------------------------------ query rows
     Walk w;
-    w.begin(p, b_first, off_first, x1 - x0);
+    if (!w.begin(p, b_first, off_first, x1 - x0)) return;
     unsigned char *q_s = smem + kOffQ;
     float *qs = reinterpret_cast<float *>(smem + kOffQs);
     int it = 0;
@@ -316,7 +327,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   const int g0 = lane >> 2, cq = lane & 3;
   const float kNegInf = -INFINITY, kNan = __int_as_float(0x7fc00000);
   Walk w;
-  w.begin(p, b_first, off_first, x1 - x0);
+  if (!w.begin(p, b_first, off_first, x1 - x0)) return;
   uint32_t g = 0;
   int it = 0;
   bool ok = true; // a wait that gave up leaves a status; the warp goes on to the end without its tiles
@@ -557,7 +568,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     if (w.i0 == 0 && tid == 0) {
       // this CTA holds the run's first tile: it says which CTAs hold the others
-      const long first = x1 - w.left; // the piece's place on the line
+      const long first = x1 - w.left; // the first tile's place on the line
       const int last = share_of(W, n, first + w.s.n_tiles - 1);
       RunInfo r;
       r.c0 = c, r.c1 = last, r.slot0 = slot, r.pad = 0;
