@@ -762,7 +762,11 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int h = 0; h < 2; ++h) {
           uint32_t o[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = hmul2(cvt_e4m3x2_f16x2((wv[2 * b8 + h][e >> 1] >> (16 * (e & 1))) & 0xffffu), fr[b8]);
+          for (int e = 0; e < 4; ++e) {
+            cvt_e4m3x4_f16x4(wv[2 * b8 + h][e], o[2 * e], o[2 * e + 1]);
+            o[2 * e] = hmul2(o[2 * e], fr[b8]);
+            o[2 * e + 1] = hmul2(o[2 * e + 1], fr[b8]);
+          }
           const uint32_t base = dst + h * kHalfTile + row * 128, c0 = 2 * (lane & 3);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + ((c0 ^ sw) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (((c0 + 1) ^ sw) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");

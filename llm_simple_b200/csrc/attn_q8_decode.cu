@@ -389,8 +389,9 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
           for (int nh = 0; nh < NH; ++nh) sc[u][nh][0] = sc[u][nh][1] = sc[u][nh][2] = sc[u][nh][3] = 0.f;
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            const uint32_t ka[4] = {cvt_e4m3x2_f16x2(kw[0][ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[1][ks] & 0xffffu), cvt_e4m3x2_f16x2(kw[0][ks] >> 16),
-                                    cvt_e4m3x2_f16x2(kw[1][ks] >> 16)};
+            uint32_t ka[4];
+            cvt_e4m3x4_f16x4(kw[0][ks], ka[0], ka[2]);
+            cvt_e4m3x4_f16x4(kw[1][ks], ka[1], ka[3]);
 #pragma unroll
             for (int nh = 0; nh < NH; ++nh) mma_16816<__half>(sc[u][nh], ka, qb[nh][ks][0], qb[nh][ks][1]);
           }
@@ -484,8 +485,9 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (int hh = 0; hh < 2; ++hh) {
               const uint32_t lo2 = __byte_perm(vw[u][0][q4], vw[u][1][q4], hh ? 0x7362 : 0x5140);
               const uint32_t hi2 = __byte_perm(vw[u][2][q4], vw[u][3][q4], hh ? 0x7362 : 0x5140);
-              const uint32_t va[4] = {cvt_e4m3x2_f16x2(lo2 & 0xffffu), cvt_e4m3x2_f16x2(lo2 >> 16), cvt_e4m3x2_f16x2(hi2 & 0xffffu),
-                                      cvt_e4m3x2_f16x2(hi2 >> 16)};
+              uint32_t va[4];
+              cvt_e4m3x4_f16x4(lo2, va[0], va[1]);
+              cvt_e4m3x4_f16x4(hi2, va[2], va[3]);
 #pragma unroll
               for (int nh = 0; nh < NH; ++nh) mma_16816<__half>(o[nh][2 * q4 + hh], va, pb[u][nh][0], pb[u][nh][1]);
             }

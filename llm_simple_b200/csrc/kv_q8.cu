@@ -149,10 +149,12 @@ template <typename T> __global__ void __launch_bounds__(kThreads) kv_read_q8_ker
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     uint32_t o[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t hpair = cvt_e4m3x2_f16x2((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
-      const float2 v = Elem<__half>::unpack(hpair);
-      o[j] = Elem<T>::pack(v.x * f, v.y * f);
+    for (int j = 0; j < 4; ++j) {
+      uint32_t lo, hi;
+      cvt_e4m3x4_f16x4(w[j], lo, hi);
+      const float2 a = Elem<__half>::unpack(lo), b2 = Elem<__half>::unpack(hi);
+      o[2 * j] = Elem<T>::pack(a.x * f, a.y * f);
+      o[2 * j + 1] = Elem<T>::pack(b2.x * f, b2.y * f);
     }
     T *dst = out + static_cast<long>(t) * p.kv_tok + h * kHeadDim + 16 * i;
     reinterpret_cast<uint4 *>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
