@@ -834,7 +834,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 }
 
 // Merges the pieces of the blocks that were cut, and zeroes the rows that see nothing.  Grid: (block and
-// KV head, groups of 32 rows); a warp takes four rows and folds their pieces in order.
+// KV head, eight rows); one warp per row.
 template <typename T> __global__ void __launch_bounds__(256) attn_q8_chunk_merge_kernel(const Q8ChunkParams cp) {
   using namespace q8c;
   const Q8AttnParams &p = cp.a;
@@ -844,32 +844,16 @@ template <typename T> __global__ void __launch_bounds__(256) attn_q8_chunk_merge
   const int u = blockIdx.x / kvH, kvh = blockIdx.x - u * kvH;
   if (u >= cp.head->n_blocks) return;
   const RunInfo info = cp.info[blockIdx.x];
-  if (info.c1 == info.c0) return; // one CTA did the whole block
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, rho = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (info.c1 == info.c0 || rho >= info.nq * G) return; // one CTA did the whole block, or the row does not exist
   const int block_rows = 2 * cp.tile_tokens * G;
-  for (int k = 0; k < 4; ++k) {
-    const int rho = blockIdx.y * 32 + warp * 4 + k;
-    if (rho >= info.nq * G) return;
-    float M = -INFINITY, Wt = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = info.c0; c <= info.c1; ++c) {
-      const long row = static_cast<long>(c == info.c0 ? info.slot0 : 2 * c) * block_rows + rho;
-      const float l = cp.lse[row];
-      const float4 v = *reinterpret_cast<const float4 *>(cp.o + row * kHeadDim + lane * 4);
-      if (l == -INFINITY) continue;
-      const float mn = fmaxf(M, l);
-      const float fa = exp2f(M - mn), fb = exp2f(l - mn);
-      Wt = Wt * fa + fb;
-      acc.x = acc.x * fa + fb * v.x, acc.y = acc.y * fa + fb * v.y, acc.z = acc.z * fa + fb * v.z, acc.w = acc.w * fa + fb * v.w;
-      M = mn;
-    }
-    if (Wt != 0.f) acc.x /= Wt, acc.y /= Wt, acc.z /= Wt, acc.w /= Wt;
-    const int tok = rho / G;
-    uint2 o;
-    o.x = Elem<T>::pack(acc.x, acc.y);
-    o.y = Elem<T>::pack(acc.z, acc.w);
-    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (static_cast<long>(info.t0) + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = o;
-  }
+  const float4 acc = join_pieces(cp.o, cp.lse, info.c1 - info.c0 + 1, lane,
+                                 [&](int i) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * block_rows + rho; });
+  const int tok = rho / G;
+  uint2 o;
+  o.x = Elem<T>::pack(acc.x, acc.y);
+  o.y = Elem<T>::pack(acc.z, acc.w);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (static_cast<long>(info.t0) + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = o;
 }
 
 namespace {
@@ -899,7 +883,7 @@ template <typename T> cudaError_t launch_typed(const Q8ChunkParams &cp, const CU
   if (e != cudaSuccess) return e;
   *launches = 1;
   const int rows = 2 * cp.tile_tokens * cp.a.group;
-  e = launch_dependent(attn_q8_chunk_merge_kernel<T>, dim3(static_cast<unsigned>(blocks * cp.a.c.n_kv_heads), (rows + 31) / 32), 256, 0, stream, cp);
+  e = launch_dependent(attn_q8_chunk_merge_kernel<T>, dim3(static_cast<unsigned>(blocks * cp.a.c.n_kv_heads), (rows + 7) / 8), 256, 0, stream, cp);
   if (e != cudaSuccess) return e;
   *launches = 2;
   return cudaGetLastError();

@@ -581,54 +581,22 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 }
 
 // Merges the pieces of the runs that were cut, and zeroes the rows that see nothing.  Grid: (sequence and
-// KV head, row); warp i folds pieces i, i + 4, ... in order, and the warps' results are joined in order.
+// KV head, four rows); one warp per row.
 template <typename T> __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8DecodeParams dp) {
   using namespace q8d;
-  __shared__ float4 xo[4][32];
-  __shared__ float2 xml[4];
   const Q8AttnParams &p = dp.a;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int kvH = p.c.n_kv_heads, G = p.group;
-  const int b = blockIdx.x / kvH, kvh = blockIdx.x - b * kvH, rho = blockIdx.y;
+  const int b = blockIdx.x / kvH, kvh = blockIdx.x - b * kvH, rho = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const RunInfo info = dp.ws.info[blockIdx.x]; // of a run without tiles: whatever was there, not used
   const Seq s = seq_of(p, b);
   if (rho >= s.nq * G) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (s.n_tiles > 0) {
-    const RunInfo info = dp.ws.info[blockIdx.x];
-    if (info.c1 <= info.c0) return;      // the run was not cut
-    const int parts = info.c1 - info.c0 + 1;
-    float M = -INFINITY, W = 0.f;
-    for (int x = warp; x < parts; x += 4) {
-      const long row = static_cast<long>(x == 0 ? info.slot0 : 2 * (info.c0 + x)) * dp.rows + rho;
-      const float l = dp.ws.lse[row];
-      const float4 v = *reinterpret_cast<const float4 *>(dp.ws.o + row * kHeadDim + lane * 4);
-      if (l == -INFINITY) continue;
-      const float mn = fmaxf(M, l);
-      const float fa = exp2f(M - mn), fb = exp2f(l - mn);
-      W = W * fa + fb;
-      acc.x = acc.x * fa + fb * v.x, acc.y = acc.y * fa + fb * v.y, acc.z = acc.z * fa + fb * v.z, acc.w = acc.w * fa + fb * v.w;
-      M = mn;
-    }
-    xo[warp][lane] = acc;
-    if (lane == 0) xml[warp] = make_float2(M, W);
-    __syncthreads();
-    if (warp != 0) return;
-    const float Mx = fmaxf(fmaxf(xml[0].x, xml[1].x), fmaxf(xml[2].x, xml[3].x));
-    float Wt = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int x = 0; x < 4; ++x) {
-      const float2 ml = xml[x];
-      if (ml.y == 0.f) continue;         // no piece, or none that sees anything
-      const float f = exp2f(ml.x - (Mx == -INFINITY ? 0.f : Mx));
-      const float4 u = xo[x][lane];
-      Wt += f * ml.y;
-      acc.x += f * u.x, acc.y += f * u.y, acc.z += f * u.z, acc.w += f * u.w;
-    }
-    if (Wt != 0.f) acc.x /= Wt, acc.y /= Wt, acc.z /= Wt, acc.w /= Wt; // NaN divides too
-  } else if (warp != 0) {
-    return;
+    if (info.c1 <= info.c0) return; // the run was not cut
+    acc = join_pieces(dp.ws.o, dp.ws.lse, info.c1 - info.c0 + 1, lane,
+                      [&](int i) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * dp.rows + rho; });
   }
   const int tok = rho / G;
   uint2 u;
@@ -659,7 +627,7 @@ cudaError_t launch_typed(const Q8DecodeParams &dp, int n_ctas, const CUtensorMap
   e = launch_dependent(attn_q8_decode_kernel<T, NH>, dim3(n_ctas), q8d::kThreads, q8d::kSmemTotal, stream, m[0], m[1], m[2], m[3], dp);
   if (e != cudaSuccess) return e;
   *launches = 1;
-  e = launch_dependent(attn_q8_merge_kernel<T>, dim3(dp.a.c.batch * dp.a.c.n_kv_heads, dp.rows), 128, 0, stream, dp);
+  e = launch_dependent(attn_q8_merge_kernel<T>, dim3(dp.a.c.batch * dp.a.c.n_kv_heads, (dp.rows + 3) / 4), 128, 0, stream, dp);
   if (e != cudaSuccess) return e;
   *launches = 2;
   return cudaGetLastError();

@@ -14,6 +14,7 @@ namespace {
 using namespace q8;
 
 constexpr int kThreads = 256;
+constexpr int kAtOnce = 4;   // rows of a thread group under way in the read kernel
 
 // Rotates the pairs of two 8-element chunks in fp32: chunks (2i, 2i + 1) for the interleaved pairing,
 // (i, i + 8) for the neox pairing.  Same products and sums as rope_pair everywhere else, no rounding
@@ -71,19 +72,35 @@ template <typename T> __global__ void __launch_bounds__(kThreads) kv_append_q8_k
   }
   const int hq = p.q_out ? p.n_heads : 0, hk = p.c.n_kv_heads;
   const int slots = hq + 2 * hk;
-  for (int first = blockIdx.z * lanes; first < slots; first += lanes * gridDim.z) {
-    const int slot = first + (grp & (lanes - 1));
-    const int which = slot < hq ? 0 : slot < hq + hk ? 1 : 2;
-    const bool on = slot < slots && (which == 0 ? table_ok : stored);
+  const int step = lanes * gridDim.z;
+  auto kind = [&](int slot) { return slot < hq ? 0 : slot < hq + hk ? 1 : 2; };                       // q, k, v
+  auto wanted = [&](int slot) { return slot < slots && (kind(slot) == 0 ? table_ok : stored); };
+  // The next row is requested before this one is worked on: a thread's 32 bytes at a time do not cover
+  // the latency of HBM.
+  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0;
+  auto request = [&](int slot) {
+    if (!wanted(slot)) return;
+    const int which = kind(slot), h = slot - (which == 0 ? 0 : which == 1 ? hq : hq + hk);
+    const bool split = which < 2 && p.is_neox; // the thread's two chunks are 64 elements apart
+    const T *src = static_cast<const T *>(which == 0 ? p.q : which == 1 ? p.k : p.v) +
+                   static_cast<long>(t) * (which == 0 ? p.q_tok : p.kv_tok) + h * kHeadDim;
+    n0 = __ldcs(reinterpret_cast<const uint4 *>(src + (split ? i : 2 * i) * 8));
+    n1 = __ldcs(reinterpret_cast<const uint4 *>(src + (split ? i + 8 : 2 * i + 1) * 8));
+  };
+  const int slot0 = blockIdx.z * lanes + (grp & (lanes - 1));
+  request(slot0);
+  for (int slot = slot0; slot - (grp & (lanes - 1)) < slots; slot += step) { // the same rounds for all lanes of a warp
+    const int which = kind(slot);
+    const bool on = wanted(slot);
     const bool rotated = which < 2;
-    const bool split = rotated && p.is_neox; // the thread's two chunks are 64 elements apart
+    const bool split = rotated && p.is_neox;
     const int c0 = split ? i : 2 * i, c1 = split ? i + 8 : 2 * i + 1;
     const int h = slot - (which == 0 ? 0 : which == 1 ? hq : hq + hk);
     float x[16];
+    const uint4 u0 = n0, u1 = n1;
+    request(slot + step);
     if (on) {
-      const T *src = static_cast<const T *>(which == 0 ? p.q : which == 1 ? p.k : p.v) +
-                     static_cast<long>(t) * (which == 0 ? p.q_tok : p.kv_tok) + h * kHeadDim;
-      unpack16<T>(__ldcs(reinterpret_cast<const uint4 *>(src + c0 * 8)), __ldcs(reinterpret_cast<const uint4 *>(src + c1 * 8)), x);
+      unpack16<T>(u0, u1, x);
       if (rotated) rotate16(x, tab, p.is_neox != 0);
     } else {
 #pragma unroll
@@ -135,30 +152,42 @@ template <typename T> __global__ void __launch_bounds__(kThreads) kv_read_q8_ker
     if (i == 0) report(p.c.error_flag, kStatusOutsideCache);
     return;
   }
-  const int hk = p.c.n_kv_heads;
-  for (int slot = (grp & (lanes - 1)) + blockIdx.z * lanes; slot < 2 * hk; slot += lanes * gridDim.z) {
-    const bool is_v = slot >= hk;
-    const int h = slot - (is_v ? hk : 0);
-    T *out = static_cast<T *>(is_v ? p.v_out : p.k_out);
-    if (!out) continue;
-    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>((is_v ? p.c.v : p.c.k) + outer * p.c.c_outer + h * p.c.c_head +
-                                                           static_cast<long>(in_pos) * p.c.c_pos + 16 * i));
-    const int x = (is_v ? p.c.vx : p.c.kx)[outer * p.c.x_outer + h * p.c.x_head + in_pos];
-    // 2^(x - 127) in two factors: x - 127 = 120 + 8 would not fit a float's exponent on its own
-    const float f = x == kPoison ? __int_as_float(0x7fc00000) : x > 0 ? pow2i(x - 127) : 0.f;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    uint32_t o[8];
+  const int hk = p.c.n_kv_heads, step = lanes * gridDim.z;
+  // several rows are under way at once: 16 bytes a thread do not cover the latency of HBM
+  for (int slot = (grp & (lanes - 1)) + blockIdx.z * lanes; slot < 2 * hk; slot += kAtOnce * step) {
+    uint4 u[kAtOnce];
+    int x[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t lo, hi;
-      cvt_e4m3x4_f16x4(w[j], lo, hi);
-      const float2 a = Elem<__half>::unpack(lo), b2 = Elem<__half>::unpack(hi);
-      o[2 * j] = Elem<T>::pack(a.x * f, a.y * f);
-      o[2 * j + 1] = Elem<T>::pack(b2.x * f, b2.y * f);
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int s = slot + k * step;
+      const bool is_v = s >= hk;
+      if (s >= 2 * hk || !(is_v ? p.v_out : p.k_out)) continue;
+      const int h = s - (is_v ? hk : 0);
+      u[k] = __ldcs(reinterpret_cast<const uint4 *>((is_v ? p.c.v : p.c.k) + outer * p.c.c_outer + h * p.c.c_head +
+                                                    static_cast<long>(in_pos) * p.c.c_pos + 16 * i));
+      x[k] = (is_v ? p.c.vx : p.c.kx)[outer * p.c.x_outer + h * p.c.x_head + in_pos];
     }
-    T *dst = out + static_cast<long>(t) * p.kv_tok + h * kHeadDim + 16 * i;
-    reinterpret_cast<uint4 *>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    reinterpret_cast<uint4 *>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int s = slot + k * step;
+      const bool is_v = s >= hk;
+      T *out = static_cast<T *>(is_v ? p.v_out : p.k_out);
+      if (s >= 2 * hk || !out) continue;
+      const float f = x[k] == kPoison ? __int_as_float(0x7fc00000) : x[k] > 0 ? pow2i(x[k] - 127) : 0.f;
+      const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t lo, hi;
+        cvt_e4m3x4_f16x4(w[j], lo, hi);
+        const float2 a = Elem<__half>::unpack(lo), b2 = Elem<__half>::unpack(hi);
+        o[2 * j] = Elem<T>::pack(a.x * f, a.y * f);
+        o[2 * j + 1] = Elem<T>::pack(b2.x * f, b2.y * f);
+      }
+      T *dst = out + static_cast<long>(t) * p.kv_tok + (s - (is_v ? hk : 0)) * kHeadDim + 16 * i;
+      __stcs(reinterpret_cast<uint4 *>(dst), make_uint4(o[0], o[1], o[2], o[3]));
+      __stcs(reinterpret_cast<uint4 *>(dst) + 1, make_uint4(o[4], o[5], o[6], o[7]));
+    }
   }
 }
 

@@ -128,6 +128,38 @@ __device__ __forceinline__ int share_of(long W, int n, long x) { return static_c
 
 } // namespace q8
 
+// Joins a row's pieces: normalised partials o[slot row][128] and log-sum-exps (log2 domain), 32 pieces a
+// round whose weights the lanes work out together; all 32 lanes, four elements each, pieces in order.
+// slot_row(i): where piece i lies.  A NaN anywhere makes the row NaN; nothing seen makes it 0.
+template <typename F>
+__device__ __forceinline__ float4 join_pieces(const float *o, const float *lse, int parts, int lane, F slot_row) {
+  float M = -INFINITY, W = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < parts; base += 32) {
+    const int n = min(32, parts - base);
+    const long row = lane < n ? slot_row(base + lane) : 0;
+    const float l = lane < n ? __ldcg(lse + row) : -INFINITY;
+    float mx = l;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    const float Mn = fmaxf(M, mx), ms = Mn == -INFINITY ? 0.f : Mn;
+    const float w = exp2f(l - ms), f = exp2f(M - ms);
+    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+    W *= f;
+    M = Mn;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const long ri = __shfl_sync(0xffffffffu, row, i);
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(o + ri * kHeadDim) + lane);
+      W += wi;
+      acc.x += wi * v.x, acc.y += wi * v.y, acc.z += wi * v.z, acc.w += wi * v.w;
+    }
+  }
+  if (W != 0.f) acc.x /= W, acc.y /= W, acc.z /= W, acc.w /= W;
+  return acc;
+}
+
 template <typename... Args>
 inline cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
