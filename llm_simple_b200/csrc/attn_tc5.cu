@@ -39,6 +39,7 @@
 #include "tc5.cuh"
 
 #include <cuda.h>
+#include <atomic>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -531,9 +532,14 @@ bool make_tensor_map_u8(CUtensorMap *map, bool swizzle, const void *base, uint64
 }
 
 int *kernel_error_word_dev() {
+  static std::atomic<int *> known[64] = {};   // the word's device address, asked for once per device
+  int dev_index = 0;
+  if (cudaGetDevice(&dev_index) != cudaSuccess || dev_index < 0 || dev_index >= 64) return nullptr;
+  if (int *dev = known[dev_index].load(std::memory_order_acquire)) return dev;
   int *w = tc5::error_word();
   int *dev = nullptr;
   if (!w || cudaHostGetDevicePointer(reinterpret_cast<void **>(&dev), w, 0) != cudaSuccess) return nullptr;
+  known[dev_index].store(dev, std::memory_order_release);
   return dev;
 }
 

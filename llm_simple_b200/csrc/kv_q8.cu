@@ -14,7 +14,14 @@ namespace {
 using namespace q8;
 
 constexpr int kThreads = 256;
-constexpr int kAtOnce = 4;   // rows of a thread group under way in the read kernel
+// CTAs per SM and rows of a thread group under way in the read kernel.  More CTAs are slower: many streams of
+// reads and writes at once cost HBM more than they hide (137,000 positions of 8 KV heads: 147 us with 3 CTAs
+// and 4 rows, 151 with 4 and 2, 171 with 6 and 2, 193 with 8 and 2).  The append kernel's values want 64 registers.
+constexpr int kAppendCtas = 4, kReadCtas = 3, kAtOnce = 4;
+// log2 of the thread groups that share a token in calls of many tokens.  A warp of the read kernel takes four
+// neighbouring positions of a head, 512 contiguous bytes of codes (eight groups per token: 180 us); the append
+// kernel reads mostly Q, whose heads are neighbours (prompts of 37 to 3900 tokens: 171 us with 0, 166 with 2).
+constexpr int kAppendLanes = 2, kReadLanes = 0;
 
 // Rotates the pairs of two 8-element chunks in fp32: chunks (2i, 2i + 1) for the interleaved pairing,
 // (i, i + 8) for the neox pairing.  Same products and sums as rope_pair everywhere else, no rounding
@@ -50,7 +57,7 @@ template <typename T> __device__ __forceinline__ uint4 pack8(const float *x) {
 
 // A group of eight threads stays with one token and walks its head rows `lanes` apart, as in
 // rope_append_kernel: the thread's share of the table row and the token's place are fetched once.
-template <typename T> __global__ void __launch_bounds__(kThreads) kv_append_q8_kernel(Q8AppendParams p, int lanes_log2) {
+template <typename T> __global__ void __launch_bounds__(kThreads, kAppendCtas) kv_append_q8_kernel(Q8AppendParams p, int lanes_log2) {
   const int i = threadIdx.x & 7, lane = threadIdx.x & 31;
   const int grp = threadIdx.x >> 3;
   const int lanes = 1 << lanes_log2;
@@ -136,7 +143,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) kv_append_q8_k
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(kThreads) kv_read_q8_kernel(Q8ReadParams p, int lanes_log2) {
+template <typename T> __global__ void __launch_bounds__(kThreads, kReadCtas) kv_read_q8_kernel(Q8ReadParams p, int lanes_log2) {
   const int i = threadIdx.x & 7, lane = threadIdx.x & 31;
   const int grp = threadIdx.x >> 3;
   const int lanes = 1 << lanes_log2;
@@ -191,10 +198,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) kv_read_q8_ker
   }
 }
 
-// Row groups per token: eight share the token's place and table row; calls of few tokens spread a
-// token's head rows over more groups, and over CTAs, so that they still fill the GPU.
-void shape_of(long tokens, int slots, int *lanes_log2, dim3 *grid) {
-  int l = 3;
+// Thread groups per token, 2^l at least: calls of few tokens spread a token's head rows over more groups,
+// and over CTAs, so that they still fill the GPU.
+void shape_of(long tokens, int slots, int l, int *lanes_log2, dim3 *grid) {
   while (l < 5 && (tokens + (32 >> l) - 1) / (32 >> l) < 148L * 8) ++l;
   while (l > 0 && (1 << (l - 1)) >= slots) --l;
   const int toks = 32 >> l;
@@ -210,7 +216,7 @@ void shape_of(long tokens, int slots, int *lanes_log2, dim3 *grid) {
 cudaError_t launch_kv_append_q8(const Q8AppendParams &p, bool bf16, cudaStream_t stream) {
   int l;
   dim3 grid;
-  shape_of(p.r.total, (p.q_out ? p.n_heads : 0) + 2 * p.c.n_kv_heads, &l, &grid);
+  shape_of(p.r.total, (p.q_out ? p.n_heads : 0) + 2 * p.c.n_kv_heads, kAppendLanes, &l, &grid);
   if (bf16) kv_append_q8_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p, l);
   else kv_append_q8_kernel<__half><<<grid, kThreads, 0, stream>>>(p, l);
   return cudaGetLastError();
@@ -219,7 +225,7 @@ cudaError_t launch_kv_append_q8(const Q8AppendParams &p, bool bf16, cudaStream_t
 cudaError_t launch_kv_read_q8(const Q8ReadParams &p, bool bf16, cudaStream_t stream) {
   int l;
   dim3 grid;
-  shape_of(p.r.total, 2 * p.c.n_kv_heads, &l, &grid);
+  shape_of(p.r.total, 2 * p.c.n_kv_heads, kReadLanes, &l, &grid);
   if (bf16) kv_read_q8_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p, l);
   else kv_read_q8_kernel<__half><<<grid, kThreads, 0, stream>>>(p, l);
   return cudaGetLastError();

@@ -225,6 +225,19 @@ def test_offsets_beyond_32_bits(ops):
         assert torch.equal(a, b) and bool(a.any())
 
 
+def test_tensors_of_another_device_are_refused(ops):
+    c = R.Cache(ops, FP16, 1, 2, 1, 64, "head")
+    x = torch.zeros((1, 2, D), dtype=torch.float16)              # in host memory: its address must not reach a kernel
+    with pytest.raises(ops.GpuOpsError, match="cpu"):
+        ops.gpu_attn_decode_q8_layer(c.desc, None, c.kv, x.cuda(), x, _i32([0]), 1, 0, 0, None, 0)
+    with pytest.raises(ops.GpuOpsError, match="cpu"):
+        ops.gpu_kv_read_q8_layer(c.desc, None, c.kv, x, None, _i32([0, 1]), None, 1)
+    with pytest.raises(ops.GpuOpsError, match="cpu"):
+        ops.gpu_rope_kv_append_q8_layer(c.desc, None, c.kv, None, None, x.cuda(), x.cuda(), x, _i32([0, 1]), _i32([0]), 1)
+    with pytest.raises(ops.GpuOpsError, match="cpu"):
+        ops.gpu_attn_chunk_q8_layer(c.desc, None, c.kv, x.cuda(), x.cuda(), torch.zeros(2, dtype=torch.int32), _i32([0]), 1, 1, 1, 0, 0, None, 0)
+
+
 # ------------------------------------------------------------------------------------------ decode
 def _decode(ops, c, q, lens, mx=None, window=0, sink=0, out=None):
     mx = mx or max(1, max(lens))
