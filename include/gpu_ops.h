@@ -396,7 +396,8 @@ int gpu_attn_decode_paged_layer(const gpu_attn_desc *desc, const gpu_kv_pages *p
  * captured graph may be replayed after they have changed.  A position outside
  * [0, max_pos) or a page id outside the pool is skipped (written nowhere; read as
  * the rows of page 0) and reported by gpu_ops_kernel_status() == 41, a length
- * beyond the host's bound == 40.
+ * beyond the host's bound == 40.  Make the first call on a device before a capture: it sets up that
+ * status word.
  * ------------------------------------------------------------------------ */
 
 /* The cache.  Codes follow the descriptor's cache strides (an element is a byte;
@@ -447,7 +448,8 @@ size_t gpu_attn_decode_q8_workspace_bytes(const gpu_attn_desc *desc, int max_kv_
 /* Causal attention of a ragged batch's new (already rotated, already appended)
  * tokens over their 8-bit caches: row r of sequence b stands at position
  * start_pos[b] + r and sees the positions up to its own, with `window` and n_sink
- * as above.  max_new: host upper bound of the new tokens of a sequence;
+ * as above.  At most 16000 sequences, unless max_new * n_heads / n_kv_heads <= 16.  max_new: host upper bound of the
+ * new tokens of a sequence (with those few rows it picks the decode kernel, otherwise it is only checked);
  * max_kv_len: of start_pos[b] + new tokens.  Rows of sequences that bring no token
  * do not exist; rows beyond the last sequence stay as they were. */
 int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages, const gpu_kv_q8 *kv, void *out,

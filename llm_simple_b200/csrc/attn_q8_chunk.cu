@@ -63,7 +63,8 @@ constexpr float kLazy = 8.0f;
 constexpr int kMaxCtas = 148;
 constexpr int kPieceCost = 6;                        // what a block costs besides its tiles, in tiles: its rows of Q, fill and drain, results.
                                                      // Prompts of 33 to 1024 tokens: 520 us with 0, 359 with 2, 312 with 4, 309 with 8
-constexpr int kMaxBatch = 16000;                     // prefix sums of the batch lie in the Q tiles while a CTA finds its share
+static_assert((kChunkMaxBatch + 1) * 4 <= 2 * 2 * 128 * 128 * 2, "prefix sums");
+// kChunkMaxBatch:                     // prefix sums of the batch lie in the Q tiles while a CTA finds its share
 
 enum { BAR_RAWFULL = 0, BAR_RAWEMPTY = 2, BAR_KFULL = 4, BAR_KEMPTY = 6, BAR_VFULL = 8, BAR_VEMPTY = 10, BAR_QFULL = 12, BAR_QTAKEN = 14,
        BAR_SFULL = 16, BAR_SFREE = 18, BAR_PFULL = 20 /* [half][x] */, BAR_ODONE = 24 /* [half][x] */, BAR_REF = 28, BAR_COUNT = 32 };
@@ -85,7 +86,7 @@ struct RunInfo {
 struct Q8ChunkParams {
   Q8AttnParams a;
   int tile_tokens;      // tokens per tile of 128 rows: 128 / group
-  int min_tiles, max_blocks;
+  int min_tiles;
   q8c::Head *head;
   q8c::RunInfo *info;   // [blocks][kv heads]
   float *o, *lse;       // [slot][2 * tile_tokens * group][128], and without the 128
@@ -266,7 +267,17 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     const int per = (p.c.batch + kThreads - 1) / kThreads;
     const int lo = min(p.c.batch, tid * per), hi = min(p.c.batch, lo + per);
     int mine = 0;
-    for (int b = lo; b < hi; ++b) mine += blocks_of(cp, b);
+    int falls = 0; // tok_start decreases somewhere: the rows overlap, and nothing below is sized for that
+    for (int b = lo; b < hi; ++b) {
+      mine += blocks_of(cp, b);
+      falls |= __ldg(p.r.tok_start + b + 1) < __ldg(p.r.tok_start + b);
+    }
+    falls = __syncthreads_or(falls);
+    if (falls) {
+      if (tid == 0) report(err, kStatusOutsideCache);
+      if (tid == 0 && blockIdx.x == 0) cp.head->n_blocks = 0;
+      return;
+    }
     int at = block_scan(mine, scan, warp, lane, n_blocks);
     for (int b = lo; b < hi; ++b) {
       prefix[b] = at;
@@ -274,10 +285,6 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     if (tid == 0) prefix[p.c.batch] = n_blocks;
     __syncthreads();
-  }
-  if (n_blocks > cp.max_blocks) { // tok_start decreases somewhere: the rows overlap
-    if (tid == 0) report(err, kStatusOutsideCache);
-    n_blocks = 0;
   }
   const int per = (n_blocks + kThreads - 1) / kThreads;
   const int u_lo = min(n_blocks, tid * per), u_hi = min(n_blocks, u_lo + per);
@@ -900,12 +907,10 @@ size_t attn_q8_chunk_ws_bytes(int batch, int n_kv_heads, int group, int total, i
 cudaError_t launch_attn_q8_chunk(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches) {
   *launches = 0;
   const Q8Cache &c = p.c;
-  if (c.batch > q8c::kMaxBatch) return cudaErrorNotSupported;
   Q8ChunkParams cp{};
   cp.a = p;
   cp.tile_tokens = 128 / p.group;
   cp.min_tiles = 1;
-  cp.max_blocks = static_cast<int>(block_bound(c.batch, p.group, p.r.total));
   const int n_ctas = chunk_ctas(c.batch, c.n_kv_heads, p.group, p.r.total, p.max_kv_len);
   const long blocks = block_bound(c.batch, p.group, p.r.total);
   char *ws = static_cast<char *>(p.ws);

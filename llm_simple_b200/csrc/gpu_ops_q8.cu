@@ -250,6 +250,8 @@ int gpu_attn_chunk_q8_layer(const gpu_attn_desc *desc, const gpu_kv_pages *pages
   if (max_new <= 0) return fail(GPU_OPS_E_INVALID, "max_new %d", max_new);
   if (int rc = check_row("q_tok_stride", desc->q_tok_stride, desc->n_heads)) return rc;
   if (int rc = check_row("out_tok_stride", desc->out_tok_stride, desc->n_heads)) return rc;
+  if (!few_rows(max_new, desc->n_heads / desc->n_kv_heads) && desc->batch > kChunkMaxBatch)
+    return fail(GPU_OPS_E_UNSUPPORTED, "batch %d: at most %d sequences", desc->batch, kChunkMaxBatch);
   if (total_tokens == 0) return GPU_OPS_OK;
   if (int rc = check_workspace(workspace, workspace_bytes, gpu_attn_chunk_q8_workspace_bytes(desc, total_tokens, max_new, max_kv_len)))
     return rc;

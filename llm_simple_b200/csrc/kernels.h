@@ -290,7 +290,8 @@ struct Q8AttnParams {
 // Up to 16 query rows per (sequence, KV head): the decode form, and chunks with max_new * group <= 16.
 cudaError_t launch_attn_q8_decode(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches);
 size_t attn_q8_decode_ws_bytes(int batch, int n_kv_heads, int rows, int max_kv_len);
-// Any number of rows: tcgen05 kernel.
+constexpr int kChunkMaxBatch = 16000;
+// Any number of rows: tcgen05 kernel; at most kChunkMaxBatch sequences.
 cudaError_t launch_attn_q8_chunk(const Q8AttnParams &p, bool bf16, cudaStream_t stream, int *launches);
 size_t attn_q8_chunk_ws_bytes(int batch, int n_kv_heads, int group, int total, int max_kv_len);
 

@@ -140,6 +140,7 @@ def test_attention(call):
         _refused(_chunk(_desc(), None, _kv(), pos=None), E_INVALID, "start_pos")
         _refused(_chunk(_desc(), None, _kv(), new=0), E_INVALID, "max_new")
         assert _chunk(_desc(), None, _kv(), total=0) == 0
+        _refused(_chunk(_desc(batch=16001), None, _kv(), new=5), E_UNSUPPORTED, "at most 16000")
     else:
         _refused(_decode(_desc(), None, _kv(), lens=None), E_INVALID, "kv_len")
 

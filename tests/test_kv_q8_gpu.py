@@ -552,6 +552,29 @@ def test_chunk_bad_bounds_are_reported(ops):
         R.assert_close(out[40:], want, tol, kind)
 
 
+def test_chunk_bad_rows_are_reported(ops):
+    """Positions before the cache see nothing; rows whose starts decrease are not computed."""
+    c = R.Cache(ops, BF16, 2, 4, 2, 128, "paged", 64)
+    c.fill([128, 43])
+    q = _randn((73, 4, D), BF16, 3)
+    out = _chunk(ops, c, q, [40, 33], [-3, 10], mx=128)
+    assert ops.gpu_ops_kernel_status() == 41
+    ops.gpu_ops_clear_kernel_status()
+    assert not bool(out[:3].any())
+    for b, rows, pos in ((0, slice(3, 40), range(37)), (1, slice(40, 73), range(10, 43))):
+        want, tol = R.attention(c, q[rows], b, list(pos), 0, 0, R.half_step(BF16))
+        R.assert_close(out[rows], want, tol)
+    for max_new in (40, 4):                                      # the tcgen05 kernel, and the one for few rows
+        n = ops.gpu_attn_chunk_q8_workspace_bytes(c.desc, 73, max_new, 128)
+        ws = torch.full((max(16, n),), 0xFF, dtype=torch.uint8, device="cuda")
+        out = torch.full_like(q, 7.0)
+        ops.gpu_attn_chunk_q8_layer(c.desc, c.pages, c.kv, out, q, _i32([0, 60, 20]), _i32([0, 0]), 73, max_new, 128, 0, 0, ws, n)
+        torch.cuda.synchronize()
+        assert ops.gpu_ops_kernel_status() in (40, 41)
+        assert bool((out[60:] == 7.0).all())
+        ops.gpu_ops_clear_kernel_status()
+
+
 def test_chunk_captured_and_replayed(ops):
     c = R.Cache(ops, BF16, 3, 4, 2, 512, "paged", 64)
     c.fill([512] * 3)
