@@ -130,7 +130,10 @@ int check_workspace(const void *workspace, size_t given, size_t need) {
   return GPU_OPS_OK;
 }
 
-// Query rows of a KV head that the decode kernel takes at once.
+// Chunks of up to 16 query rows of a KV head go to the decode kernel, which takes that many at once; the
+// tcgen05 kernel pays for 128 at least.  Measured on both: 16 sequences of 4000 to 8000 positions, 40 / 8 heads,
+// 3 tokens each: 71 against 123 us; 8 sequences of up to 3000, 16 MHA heads, 16 tokens: 36 against 60.  More rows
+// in several walks over the cache do not pay: 6 tokens of the first case 118 against 125 us, 9 tokens 165 against 127.
 bool few_rows(int max_new, int group) { return static_cast<long>(max_new) * group <= 16; }
 
 float scale_log2_of_128() { return (1.0f / sqrtf(128.0f)) * 1.4426950408889634f; }
