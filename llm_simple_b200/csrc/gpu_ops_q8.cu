@@ -89,10 +89,16 @@ int cache_from(const gpu_attn_desc *d, const gpu_kv_pages *pages, const gpu_kv_q
   // rows, heads and sequences (pages) may be nested in any order, but must not overlap
   if (c->c_pos < 128 || (d->n_kv_heads > 1 && c->c_head < 128) || (outers > 1 && c->c_outer < 128) || c->c_head < 0 || c->c_outer < 0)
     return fail(GPU_OPS_E_INVALID, "cache strides: outer %ld, head %ld, position %ld", c->c_outer, c->c_head, c->c_pos);
+  // (a dimension whose stride is the larger one has to clear what lies inside it)
+  const long all_rows = (rows - 1) * c->c_pos + 128, all_heads = (d->n_kv_heads - 1) * c->c_head + 128;
+  const bool heads_outside = c->c_head > c->c_pos;
+  if (d->n_kv_heads > 1 && (heads_outside ? all_rows > c->c_head : rows > 1 && all_heads > c->c_pos))
+    return fail(GPU_OPS_E_INVALID, "%ld positions do not fit the cache (head stride %ld, position stride %ld)", rows, c->c_head, c->c_pos);
   const long widest = c->c_pos > c->c_head ? c->c_pos : c->c_head;
-  if (outers > 1 && c->c_outer >= widest && rows * d->n_kv_heads * 128 > c->c_outer)
-    return fail(GPU_OPS_E_INVALID, "%ld positions do not fit the cache (%ld per %s)", rows, c->c_outer / (128L * d->n_kv_heads),
-                pages ? "page" : "sequence");
+  const long extent = all_rows + (d->n_kv_heads - 1) * c->c_head;
+  if (outers > 1 && c->c_outer >= widest && extent > c->c_outer)
+    return fail(GPU_OPS_E_INVALID, "%ld positions do not fit the cache (%ld bytes, the next %s begins at %ld)", rows, extent,
+                pages ? "page" : "sequence", c->c_outer);
   const long padded = (rows + 15) / 16 * 16;
   if ((d->n_kv_heads > 1 && c->x_head < padded) || (outers > 1 && c->x_outer < padded) || c->x_head < 0 || c->x_outer < 0)
     return fail(GPU_OPS_E_INVALID, "exponent strides: outer %ld, head %ld; rows of %ld bytes", c->x_outer, c->x_head, padded);

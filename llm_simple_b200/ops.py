@@ -435,7 +435,7 @@ def _on_current_device(*tensors):
 def gpu_rope_kv_append_q8_layer(desc, pages, kv, q_out, q_in, k_in, v_in, freqs_cis, tok_start_dev, start_pos_dev,
                                 total_tokens, stream=None):
     """RoPE + append of a ragged batch into an 8-bit cache (make_kv_q8); pages: None for a flat cache."""
-    _on_current_device(q_out, q_in, k_in, v_in, freqs_cis, tok_start_dev, start_pos_dev, getattr(kv, "_keep", (None,))[0])
+    _on_current_device(q_out, q_in, k_in, v_in, freqs_cis, tok_start_dev, start_pos_dev, getattr(kv, "_keep", (None,))[0], getattr(pages, "_keep", None))
     _check(lib().gpu_rope_kv_append_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(q_out), _ptr(q_in),
                                              _ptr(k_in), _ptr(v_in), _ptr(freqs_cis), _ptr(tok_start_dev),
                                              _ptr(start_pos_dev), total_tokens, _stream(stream)))
@@ -443,7 +443,7 @@ def gpu_rope_kv_append_q8_layer(desc, pages, kv, q_out, q_in, k_in, v_in, freqs_
 
 def gpu_kv_read_q8_layer(desc, pages, kv, k_out, v_out, tok_start_dev, start_pos_dev, total_tokens, stream=None):
     """Rows of an 8-bit cache back in 16 bits, ragged; start_pos_dev None: from position 0."""
-    _on_current_device(k_out, v_out, tok_start_dev, start_pos_dev, getattr(kv, "_keep", (None,))[0])
+    _on_current_device(k_out, v_out, tok_start_dev, start_pos_dev, getattr(kv, "_keep", (None,))[0], getattr(pages, "_keep", None))
     _check(lib().gpu_kv_read_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(k_out), _ptr(v_out),
                                       _ptr(tok_start_dev), _ptr(start_pos_dev), total_tokens, _stream(stream)))
 
@@ -455,7 +455,7 @@ def gpu_attn_decode_q8_workspace_bytes(desc, max_kv_len):
 def gpu_attn_decode_q8_layer(desc, pages, kv, out, q, kv_len_dev, max_kv_len, window, n_sink, workspace,
                              workspace_bytes, stream=None):
     """One rotated query row per sequence over its 8-bit cache; window 0: everything is visible."""
-    _on_current_device(out, q, kv_len_dev, workspace, getattr(kv, "_keep", (None,))[0])
+    _on_current_device(out, q, kv_len_dev, workspace, getattr(kv, "_keep", (None,))[0], getattr(pages, "_keep", None))
     _check(lib().gpu_attn_decode_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(out), _ptr(q),
                                           _ptr(kv_len_dev), max_kv_len, window, n_sink, _ptr(workspace),
                                           workspace_bytes, _stream(stream)))
@@ -468,7 +468,7 @@ def gpu_attn_chunk_q8_workspace_bytes(desc, total_tokens, max_new, max_kv_len):
 def gpu_attn_chunk_q8_layer(desc, pages, kv, out, q, tok_start_dev, start_pos_dev, total_tokens, max_new, max_kv_len,
                             window, n_sink, workspace, workspace_bytes, stream=None):
     """Causal attention of a ragged batch's new, appended tokens over their 8-bit caches."""
-    _on_current_device(out, q, tok_start_dev, start_pos_dev, workspace, getattr(kv, "_keep", (None,))[0])
+    _on_current_device(out, q, tok_start_dev, start_pos_dev, workspace, getattr(kv, "_keep", (None,))[0], getattr(pages, "_keep", None))
     _check(lib().gpu_attn_chunk_q8_layer(ctypes.byref(desc), _ref(pages), _ref(kv), _ptr(out), _ptr(q),
                                          _ptr(tok_start_dev), _ptr(start_pos_dev), total_tokens, max_new, max_kv_len,
                                          window, n_sink, _ptr(workspace), workspace_bytes, _stream(stream)))

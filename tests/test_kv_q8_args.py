@@ -81,6 +81,15 @@ def test_cache(call):
     _refused(call(_desc(), None, _kv(head=240)), E_INVALID, "exponent strides")
     _refused(call(_desc(), None, _kv(head=264)), E_INVALID, "multiples of 16")
     _refused(call(_desc(), None, _kv(outer=496)), E_INVALID, "exponent rows")
+    one = _desc(batch=1)                                          # one sequence: its positions must not run into the next head
+    _refused(call(one, None, _kv(max_pos=257, head=272)), E_INVALID, "do not fit the cache")
+    _refused(call(_desc(batch=1, layout="token", H=8, kvH=2, cap=256), None, _kv(max_pos=0)), E_INVALID, "max_pos")
+    d = _desc(layout="token")
+    d.cache_head_stride = 256                                     # two heads of 128 bytes in a position of 256
+    _refused(call(d, None, _kv()), E_INVALID, "do not fit the cache")
+    d = _desc(layout="token")
+    d.cache_pos_stride = 512                                      # positions twice as far apart, sequences not
+    _refused(call(d, None, _kv()), E_INVALID, "do not fit the cache")
     for field, value in (("cache_pos_stride", 136), ("cache_head_stride", 256 * 128 + 8), ("cache_seq_stride", 2 * 256 * 128 + 8)):
         d = _desc()
         setattr(d, field, value)

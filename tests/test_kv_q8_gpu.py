@@ -287,7 +287,8 @@ def test_decode_long(ops, batch, kvH, n):
     for b in sorted({0, 1, batch // 2, batch - 1} & set(range(batch))):
         want, tol = R.attention(c, q[b:b + 1], b, [lens[b] - 1], 0, 0, R.half_step(FP16))
         R.assert_close(out[b:b + 1], want, tol, "sequence %d" % b)
-    assert torch.equal(out, _decode(ops, c, q, lens))            # the same bits every time
+    for _ in range(10):
+        assert torch.equal(out, _decode(ops, c, q, lens))        # the same bits every time
 
 
 def test_decode_unseen_pages_need_not_exist(ops):
@@ -598,6 +599,42 @@ def test_chunk_captured_and_replayed(ops):
         g.replay()
         torch.cuda.synchronize()
         _check_chunk(c, q, out, new, st, 0, 0, "replay")
+
+
+def test_two_streams_at_once(ops):
+    """Calls that overlap on the GPU, each with a workspace of its own, give what they give alone."""
+    H, kvH, n = 8, 2, 3000
+    c = R.Cache(ops, BF16, 8, H, kvH, n, "paged", 64)
+    c.fill([n - 100 * b for b in range(8)])
+    lens = _i32([n - 100 * b for b in range(8)])
+    qd, qc = _randn((8, H, D), BF16, 3), _randn((8 * 40, H, D), BF16, 4)
+    tok, start = _i32(np.arange(9) * 40), lens - 40
+    n_d = ops.gpu_attn_decode_q8_workspace_bytes(c.desc, n)
+    n_c = ops.gpu_attn_chunk_q8_workspace_bytes(c.desc, 320, 40, n)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    ws = [torch.empty(max(n_d, n_c), dtype=torch.uint8, device="cuda") for _ in streams]
+    outs = [torch.zeros_like(qc if i % 2 else qd) for i in range(4)]
+
+    def call(i):
+        if i % 2:
+            ops.gpu_attn_chunk_q8_layer(c.desc, c.pages, c.kv, outs[i], qc, tok, start, 320, 40, n, 0, 0, ws[i], n_c)
+        else:
+            ops.gpu_attn_decode_q8_layer(c.desc, c.pages, c.kv, outs[i], qd, lens, n, 0, 0, ws[i], n_d)
+
+    want = []
+    for i in range(2):
+        call(i)
+        torch.cuda.synchronize()
+        want.append(outs[i].clone())
+        outs[i].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                call(i)
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert torch.equal(outs[i], want[i % 2])
 
 
 # ------------------------------------------------------------------------------------------ together
