@@ -322,15 +322,16 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         scan[17] = u - prefix[b];
         scan[18] = static_cast<int>(x0 - at);
       }
-      for (int h = 0; h < kvH; ++h) { // the CTAs share the writing of the merge's records
-        if ((static_cast<unsigned>(u) * kvH + h) % gridDim.x != c) continue;
+      // the CTAs share the writing of the merge's records: this one has those of number c, c + grid, ...
+      const int ctas = static_cast<int>(gridDim.x), ahead = c - static_cast<int>(static_cast<unsigned>(u) * kvH % gridDim.x);
+      for (int h = ahead < 0 ? ahead + ctas : ahead; h < kvH; h += ctas) {
         RunInfo r{};
         r.c1 = -1;
         if (s.n_tiles > 0) {
           const long first = at + static_cast<long>(h) * one;
           r.c0 = share_of(W, n, first + kPieceCost);
           r.c1 = share_of(W, n, first + one - 1);
-          r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) >= first ? 0 : 1);
+            r.slot0 = 2 * r.c0 + (share_begin(W, n, r.c0) >= first ? 0 : 1);
         }
         r.t0 = s.t0;
         r.nq = s.nq;
