@@ -841,9 +841,8 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   }
 }
 
-// Merges the pieces of the blocks that were cut, and zeroes the rows that see nothing.  Grid: (block and
-// KV head, eight rows); one warp per row.
-template <typename T> __global__ void __launch_bounds__(256) attn_q8_chunk_merge_kernel(const Q8ChunkParams cp) {
+// Merges the pieces of the blocks that were cut, and zeroes the rows that see nothing.
+template <typename T> __global__ void __launch_bounds__(32 * kMergeWarps) attn_q8_chunk_merge_kernel(const Q8ChunkParams cp, int split) {
   using namespace q8c;
   const Q8AttnParams &p = cp.a;
   cudaTriggerProgrammaticLaunchCompletion();
@@ -852,16 +851,18 @@ template <typename T> __global__ void __launch_bounds__(256) attn_q8_chunk_merge
   const int u = blockIdx.x / kvH, kvh = blockIdx.x - u * kvH;
   if (u >= cp.head->n_blocks) return;
   const RunInfo info = cp.info[blockIdx.x];
-  const int lane = threadIdx.x & 31, rho = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (info.c1 == info.c0 || rho >= info.nq * G) return; // one CTA did the whole block, or the row does not exist
+  if (info.c1 == info.c0) return; // one CTA did the whole block
   const int block_rows = 2 * cp.tile_tokens * G;
-  const float4 acc = join_pieces(cp.o, cp.lse, info.c1 - info.c0 + 1, lane,
-                                 [&](int i) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * block_rows + rho; });
-  const int tok = rho / G;
-  uint2 o;
-  o.x = Elem<T>::pack(acc.x, acc.y);
-  o.y = Elem<T>::pack(acc.z, acc.w);
-  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (static_cast<long>(info.t0) + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = o;
+  merge_rows(cp.o, cp.lse, info.c1 - info.c0 + 1, info.nq * G, split,
+             [&](int i, int rho) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * block_rows + rho; },
+             [&](int rho, const float4 &v) {
+               const int tok = rho / G;
+               uint2 o;
+               o.x = Elem<T>::pack(v.x, v.y);
+               o.y = Elem<T>::pack(v.z, v.w);
+               *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + (static_cast<long>(info.t0) + tok) * p.out_row +
+                                          (kvh * G + rho - tok * G) * kHeadDim + (threadIdx.x & 31) * 4) = o;
+             });
 }
 
 namespace {
@@ -890,8 +891,10 @@ template <typename T> cudaError_t launch_typed(const Q8ChunkParams &cp, const CU
   e = launch_dependent(attn_q8_chunk_kernel<T>, dim3(n_ctas), q8c::kThreads, q8c::kSmemTotal, stream, mk, mv, cp);
   if (e != cudaSuccess) return e;
   *launches = 1;
-  const int rows = 2 * cp.tile_tokens * cp.a.group;
-  e = launch_dependent(attn_q8_chunk_merge_kernel<T>, dim3(static_cast<unsigned>(blocks * cp.a.c.n_kv_heads), (rows + 7) / 8), 256, 0, stream, cp);
+  dim3 grid;
+  int split;
+  merge_shape(blocks * cp.a.c.n_kv_heads, 2 * cp.tile_tokens * cp.a.group, n_ctas, &grid, &split);
+  e = launch_dependent(attn_q8_chunk_merge_kernel<T>, grid, 32 * kMergeWarps, 0, stream, cp, split);
   if (e != cudaSuccess) return e;
   *launches = 2;
   return cudaGetLastError();

@@ -580,29 +580,27 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   } while (w.next(p));
 }
 
-// Merges the pieces of the runs that were cut, and zeroes the rows that see nothing.  Grid: (sequence and
-// KV head, four rows); one warp per row.
-template <typename T> __global__ void __launch_bounds__(128) attn_q8_merge_kernel(const Q8DecodeParams dp) {
+// Merges the pieces of the runs that were cut, and zeroes the rows that see nothing.
+template <typename T> __global__ void __launch_bounds__(32 * kMergeWarps) attn_q8_merge_kernel(const Q8DecodeParams dp, int split) {
   using namespace q8d;
   const Q8AttnParams &p = dp.a;
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int kvH = p.c.n_kv_heads, G = p.group;
-  const int b = blockIdx.x / kvH, kvh = blockIdx.x - b * kvH, rho = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int b = blockIdx.x / kvH, kvh = blockIdx.x - b * kvH;
   const RunInfo info = dp.ws.info[blockIdx.x]; // of a run without tiles: whatever was there, not used
   const Seq s = seq_of(p, b);
-  if (rho >= s.nq * G) return;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (s.n_tiles > 0) {
-    if (info.c1 <= info.c0) return; // the run was not cut
-    acc = join_pieces(dp.ws.o, dp.ws.lse, info.c1 - info.c0 + 1, lane,
-                      [&](int i) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * dp.rows + rho; });
-  }
-  const int tok = rho / G;
-  uint2 u;
-  u.x = Elem<T>::pack(acc.x, acc.y);
-  u.y = Elem<T>::pack(acc.z, acc.w);
-  *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + static_cast<long>(s.t0 + tok) * p.out_row + (kvh * G + rho - tok * G) * kHeadDim + lane * 4) = u;
+  if (s.n_tiles > 0 && info.c1 <= info.c0) return; // the run was not cut
+  merge_rows(dp.ws.o, dp.ws.lse, s.n_tiles > 0 ? info.c1 - info.c0 + 1 : 0, s.nq * G, split,
+             [&](int i, int rho) { return static_cast<long>(i == 0 ? info.slot0 : 2 * (info.c0 + i)) * dp.rows + rho; },
+             [&](int rho, const float4 &v) {
+               const int tok = rho / G;
+               uint2 u;
+               u.x = Elem<T>::pack(v.x, v.y);
+               u.y = Elem<T>::pack(v.z, v.w);
+               *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + static_cast<long>(s.t0 + tok) * p.out_row +
+                                          (kvh * G + rho - tok * G) * kHeadDim + (threadIdx.x & 31) * 4) = u;
+             });
 }
 
 namespace {
@@ -627,7 +625,10 @@ cudaError_t launch_typed(const Q8DecodeParams &dp, int n_ctas, const CUtensorMap
   e = launch_dependent(attn_q8_decode_kernel<T, NH>, dim3(n_ctas), q8d::kThreads, q8d::kSmemTotal, stream, m[0], m[1], m[2], m[3], dp);
   if (e != cudaSuccess) return e;
   *launches = 1;
-  e = launch_dependent(attn_q8_merge_kernel<T>, dim3(dp.a.c.batch * dp.a.c.n_kv_heads, (dp.rows + 3) / 4), 128, 0, stream, dp);
+  dim3 grid;
+  int split;
+  merge_shape(static_cast<long>(dp.a.c.batch) * dp.a.c.n_kv_heads, dp.rows, n_ctas, &grid, &split);
+  e = launch_dependent(attn_q8_merge_kernel<T>, grid, 32 * kMergeWarps, 0, stream, dp, split);
   if (e != cudaSuccess) return e;
   *launches = 2;
   return cudaGetLastError();

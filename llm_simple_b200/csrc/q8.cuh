@@ -135,36 +135,93 @@ __device__ __forceinline__ int share_of(long W, int n, long x) {
 
 } // namespace q8
 
-// Joins a row's pieces: normalised partials o[slot row][128] and log-sum-exps (log2 domain), 32 pieces a
-// round whose weights the lanes work out together; all 32 lanes, four elements each, pieces in order.
-// slot_row(i): where piece i lies.  A NaN anywhere makes the row NaN; nothing seen makes it 0.
+// Joins pieces [begin, end) of a row: normalised partials o[slot row][128] and log-sum-exps (log2 domain), 32
+// pieces a round whose weights the lanes work out together; all 32 lanes, four elements each, pieces in order.
+// slot_row(i): where piece i lies.  The result is acc / W at the maximum M; a NaN anywhere makes it NaN.
+struct Joined {
+  float4 acc;
+  float M, W;
+};
 template <typename F>
-__device__ __forceinline__ float4 join_pieces(const float *o, const float *lse, int parts, int lane, F slot_row) {
-  float M = -INFINITY, W = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = 0; base < parts; base += 32) {
-    const int n = min(32, parts - base);
+__device__ __forceinline__ Joined join_pieces(const float *o, const float *lse, int begin, int end, int lane, F slot_row) {
+  Joined r;
+  r.M = -INFINITY, r.W = 0.f;
+  r.acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = begin; base < end; base += 32) {
+    const int n = min(32, end - base);
     const long row = lane < n ? slot_row(base + lane) : 0;
     const float l = lane < n ? __ldcg(lse + row) : -INFINITY;
     float mx = l;
 #pragma unroll
     for (int d = 16; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float Mn = fmaxf(M, mx), ms = Mn == -INFINITY ? 0.f : Mn;
-    const float w = exp2f(l - ms), f = exp2f(M - ms);
-    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-    W *= f;
-    M = Mn;
+    const float Mn = fmaxf(r.M, mx), ms = Mn == -INFINITY ? 0.f : Mn;
+    const float w = exp2f(l - ms), f = exp2f(r.M - ms);
+    r.acc.x *= f, r.acc.y *= f, r.acc.z *= f, r.acc.w *= f;
+    r.W *= f;
+    r.M = Mn;
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
       const float wi = __shfl_sync(0xffffffffu, w, i);
       const long ri = __shfl_sync(0xffffffffu, row, i);
       const float4 v = __ldcg(reinterpret_cast<const float4 *>(o + ri * kHeadDim) + lane);
-      W += wi;
-      acc.x += wi * v.x, acc.y += wi * v.y, acc.z += wi * v.z, acc.w += wi * v.w;
+      r.W += wi;
+      r.acc.x += wi * v.x, r.acc.y += wi * v.y, r.acc.z += wi * v.z, r.acc.w += wi * v.w;
     }
   }
-  if (W != 0.f) acc.x /= W, acc.y /= W, acc.z /= W, acc.w /= W;
-  return acc;
+  return r;
+}
+
+// The rows of one cut run: a CTA of eight warps, `split` of them on a row, takes rows blockIdx.y * 8 / split ..
+// and so on, gridDim.y CTAs apart.  store(rho, four elements of this lane).
+constexpr int kMergeWarps = 8;
+template <typename F, typename S>
+__device__ __forceinline__ void merge_rows(const float *o, const float *lse, int parts, int rows, int split, F slot_row, S store) {
+  __shared__ float4 xo[kMergeWarps][32];
+  __shared__ float2 xml[kMergeWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % split, per = kMergeWarps / split;
+  for (int r0 = blockIdx.y * per; r0 < rows; r0 += gridDim.y * per) {
+    const int rho = r0 + warp / split;
+    Joined j;
+    j.acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    j.M = -INFINITY, j.W = 0.f;
+    if (rho < rows)
+      j = join_pieces(o, lse, parts * sub / split, parts * (sub + 1) / split, lane, [&](int i) { return slot_row(i, rho); });
+    if (split > 1) {
+      xo[warp][lane] = j.acc;
+      if (lane == 0) xml[warp] = make_float2(j.M, j.W);
+      __syncthreads();
+      if (sub == 0) {
+        float M = -INFINITY;
+        for (int x = 0; x < split; ++x) M = fmaxf(M, xml[warp + x].x);
+        const float ms = M == -INFINITY ? 0.f : M;
+        j.acc = make_float4(0.f, 0.f, 0.f, 0.f), j.W = 0.f;
+        for (int x = 0; x < split; ++x) {
+          const float2 ml = xml[warp + x];
+          if (ml.y == 0.f) continue;     // no piece, or none that sees anything
+          const float f = exp2f(ml.x - ms);
+          const float4 u = xo[warp + x][lane];
+          j.W += f * ml.y;
+          j.acc.x += f * u.x, j.acc.y += f * u.y, j.acc.z += f * u.z, j.acc.w += f * u.w;
+        }
+      }
+      __syncthreads();
+    }
+    if (sub == 0 && rho < rows) {
+      if (j.W != 0.f) j.acc.x /= j.W, j.acc.y /= j.W, j.acc.z /= j.W, j.acc.w /= j.W; // NaN divides too
+      store(rho, j.acc);
+    }
+  }
+}
+// Grid and split of a merge over `runs` runs of `rows` rows, cut for `ctas` CTAs: enough CTAs to fill the GPU,
+// few enough that those of runs that were not cut leave soon (ragged prompts, 640 runs: 347 us in all with 512 / runs
+// CTAs a run, 305 with 2048, 298 with 4096); several warps on a row where a run can have many pieces (20 tokens of 6
+// heads behind 30000 positions, 74 pieces: the call takes 67 us with a warp per row, 31 so).
+inline void merge_shape(long runs, int rows, int ctas, dim3 *grid, int *split) {
+  *split = ctas >= 16 * runs ? 8 : ctas >= 8 * runs ? 4 : 1;
+  const long per = kMergeWarps / *split, most = (rows + per - 1) / per;
+  long gy = (4096 + runs - 1) / runs;
+  gy = gy > most ? most : gy < 1 ? 1 : gy;
+  *grid = dim3(static_cast<unsigned>(runs), static_cast<unsigned>(gy));
 }
 
 template <typename... Args>
