@@ -25,9 +25,15 @@
 // exponent says "not finite" becomes a NaN row of K' and zeros in V', so that exactly the rows that
 // see it turn NaN.
 //
-// Bound by the tensor pipe and, equally, the exponentials: 128 x 128 x 16 products take 64 cycles, so
-// a tile of 128 positions against 256 rows takes 2048 cycles, as do its 32768 exponentials at 16 a
-// cycle.
+// A tile is taken in two steps of 64 positions: the softmax warps copy a step's scores to registers and
+// free them at once, so that the next step's Q K^T runs while they work.  Tensor memory: S_A, S_B 64
+// columns each, P_A, P_B two halves of 32, O_A, O_B 128.
+//
+// A tile of 128 positions against 256 rows is 2048 cycles of products (63 cycles for 128 x 128 x 16, about
+// 50 for the 128 x 64 x 16 of Q K^T, which shared memory feeds) and 2048 of exponentials (16 a cycle).
+// Measured 4900: 4096 tokens behind 12288, 40 / 8 heads, 1450 us (830 TFLOP/s).  What bounds it is the
+// softmax warps: two on a scheduler, an instruction of each every four to five cycles; without the products
+// they take 1270 us, the products and barriers alone 925, the converters 940.
 #include "q8.cuh"
 #include "tc5.cuh"
 #include "tma.cuh"
@@ -86,7 +92,6 @@ struct RunInfo {
 struct Q8ChunkParams {
   Q8AttnParams a;
   int tile_tokens;      // tokens per tile of 128 rows: 128 / group
-  int min_tiles;
   q8c::Head *head;
   q8c::RunInfo *info;   // [blocks][kv heads]
   float *o, *lse;       // [slot][2 * tile_tokens * group][128], and without the 128
@@ -306,7 +311,7 @@ attn_q8_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   int total;
   const int before = block_scan(mine, scan, warp, lane, total);
   const long W = static_cast<long>(total) * kvH;
-  const int n = static_cast<int>(min(static_cast<long>(gridDim.x), (W + cp.min_tiles - 1) / cp.min_tiles));
+  const int n = static_cast<int>(min(static_cast<long>(gridDim.x), W));
   const int c = blockIdx.x;
   const long x0 = c < n ? share_begin(W, n, c) : -1, x1 = c < n ? share_begin(W, n, c + 1) : -1;
   if (c == 0 && tid == 0) cp.head->n_blocks = n_blocks;
@@ -914,7 +919,6 @@ cudaError_t launch_attn_q8_chunk(const Q8AttnParams &p, bool bf16, cudaStream_t 
   Q8ChunkParams cp{};
   cp.a = p;
   cp.tile_tokens = 128 / p.group;
-  cp.min_tiles = 1;
   const int n_ctas = chunk_ctas(c.batch, c.n_kv_heads, p.group, p.r.total, p.max_kv_len);
   const long blocks = block_bound(c.batch, p.group, p.r.total);
   char *ws = static_cast<char *>(p.ws);
